@@ -389,6 +389,96 @@ int ms_expert_mlp_static(const ms_geom* geom, const void* arena, int n_slots,
  * status. Allocates nothing either. */
 int ms_expert_mlp_static_status(void* stream);
 
+/* ---------------------------------------------- block-scaled fp8 operators
+ * No counterpart in the reference, whose experts are 4-bit affine. The
+ * format is that of fp8 checkpoints of these models: e4m3 codes and fp32
+ * scales, value = code * scale, weights with one scale per 128 x 128 block
+ * (scales [ceil(n/128)][ceil(k/128)] of a matrix [n][k]), activations with
+ * one per row and 128 consecutive features (scales [T][ceil(d/128)]). The
+ * last block of a row or column may be smaller.
+ *
+ * Every call reads an argument block, enqueues on `stream` on device
+ * `device` (whatever the current one is), allocates nothing and does not
+ * synchronise; it can be captured. Calls share no state, so they may run at
+ * once on several streams or host threads. Strides count elements between
+ * rows; rows themselves are contiguous. A call over no rows does nothing. */
+#define MS_DT_BF16        0
+#define MS_DT_F16         1
+#define MS_DT_F32         2
+#define MS_FP8_MAX_FEATURES 16384
+#define MS_FP8_MAX_TOKENS 64
+
+/* Residual add, RMSNorm and quantisation (the norm and residual of
+ * ms_moe_block_fused, with an 8-bit output), per row of d features:
+ *   h = round(x + residual) to dtype            (h = x without residual)
+ *   y = h / sqrt(mean(h^2) + eps) * weight      (squares summed in 64 bits)
+ *   per 128 features: a = max(max|y|, 2^-100), scale = the smallest power of
+ *   two with a <= 448 scale, q = e4m3(y / scale); scale and codes are NaN
+ *   where a is not finite.
+ * weight NULL quantises x itself (then residual, h and y are NULL too). y is
+ * optional: the normalised rows, rounded to dtype. h may be x or residual;
+ * no other buffers may overlap. */
+typedef struct ms_fp8_norm {
+  const void* x;            /* dtype [T, d]                                        */
+  const void* residual;     /* dtype [T, d] or NULL                                */
+  const void* weight;       /* dtype [d] or NULL                                   */
+  void* h;                  /* dtype [T, d]; NULL only without residual            */
+  void* y;                  /* dtype [T, d] or NULL                                */
+  void* q;                  /* e4m3 [T, d]                                         */
+  float* scales;            /* [T, ceil(d/128)], contiguous                        */
+  int64_t x_stride, residual_stride, h_stride, y_stride, q_stride;
+  double eps;
+  int32_t T, d, dtype, device;
+} ms_fp8_norm;
+int ms_rms_norm_fp8(const ms_fp8_norm* args, void* stream);
+
+/* y[m][n] = sum_b x_scales[m][b] w_scales[n/128][b]
+ *           sum_{k in block b} x[m][k] w[n][k]  (+ bias[n]),
+ * sums in 32 bits, one rounding to out_dtype. Rows of x and w start on
+ * 16-byte boundaries (pad the stride when K is not a multiple of 16; what
+ * lies between K and the stride is not used). */
+typedef struct ms_fp8_linear {
+  const void* x;            /* e4m3 [M, K]                                         */
+  const float* x_scales;    /* [M, ceil(K/128)]                                    */
+  const void* w;            /* e4m3 [N, K]                                         */
+  const float* w_scales;    /* [ceil(N/128), ceil(K/128)], contiguous              */
+  const float* bias;        /* [N] or NULL                                         */
+  void* y;                  /* out_dtype [M, N]                                    */
+  int64_t x_stride, x_scales_stride, w_stride, y_stride;
+  int32_t M, N, K, out_dtype, device, reserved;
+} ms_fp8_linear;
+int ms_linear_fp8(const ms_fp8_linear* args, void* stream);
+
+/* A whole MoE layer for up to MS_FP8_MAX_TOKENS tokens over resident fp8
+ * experts (ms_moe_block's arithmetic without its pool):
+ *   logits = x router^T (+ router_bias), 32 bits;
+ *   MS_MODEL_QWEN3: softmax over the experts, the top_k largest (ties to the
+ *   lower index), renormalised if norm_topk_prob; MS_MODEL_GPTOSS: the top_k
+ *   largest logits, softmax of those;
+ *   x and the activations are quantised as in ms_rms_norm_fp8;
+ *   g, u = gate and up products (+ biases); act = silu(g) u, or for gpt-oss
+ *   with g = min(g, 7), u = clamp(u, -7, 7): g sigmoid(1.702 g) (u + 1);
+ *   y = sum_j p_j (down product_j (+ bias)) (+ residual), bf16.
+ * codes, scales, bias: gate, up [n_experts][d_ff][d_model] and down
+ * [n_experts][d_model][d_ff], contiguous. y may be x or residual. workspace:
+ * ms_moe_fp8_workspace bytes of device memory (it reads the sizes alone), for
+ * this call alone until it has run; it needs no initialisation. */
+typedef struct ms_fp8_moe {
+  const void* x;            /* bf16 [T, d_model]                                   */
+  const void* router;       /* bf16 [n_experts, d_model]                           */
+  const float* router_bias; /* [n_experts] or NULL                                 */
+  const void* codes[3];     /* gate, up, down: e4m3                                */
+  const float* scales[3];
+  const float* bias[3];     /* [n_experts][d_ff, d_ff, d_model] or NULL            */
+  const void* residual;     /* bf16 [T, d_model] or NULL                           */
+  void* y;                  /* bf16 [T, d_model]                                   */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t model, T, d_model, d_ff, n_experts, top_k, norm_topk_prob, device;
+} ms_fp8_moe;
+int ms_moe_fp8_workspace(const ms_fp8_moe* args, size_t* bytes);
+int ms_moe_fp8_layer(const ms_fp8_moe* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,7 +3,9 @@
 Host side in Python over a C-ABI CUDA library (libmoestream.so, sm_100a).
 The public surface mirrors the reference's: ``ExpertPool`` (engine_v3.py
 ExpertPool), ``MoEBlock`` / ``streaming_call`` (the patched block call), and
-``expert_mlp`` (kernels.moe_expert_mlp).
+``expert_mlp`` (kernels.moe_expert_mlp). ``fp8`` holds the operators of
+block-scaled e4m3 models: ``rms_norm_fp8``, ``quantize_fp8``, ``Fp8Linear``
+and ``Fp8MoELayer``.
 """
 from . import geometry, store
 from .geometry import Geometry, qwen3, gptoss
@@ -18,4 +20,7 @@ def __getattr__(name):
     if name in ("MoEBlock", "streaming_call", "route", "expert_mlp", "block_debug"):
         from . import block
         return getattr(block, name)
+    if name in ("rms_norm_fp8", "quantize_fp8", "quantize_weight_fp8", "Fp8Linear", "Fp8MoELayer"):
+        from . import fp8
+        return getattr(fp8, name)
     raise AttributeError(name)

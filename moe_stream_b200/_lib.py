@@ -109,6 +109,10 @@ EXPORTS = {
     "ms_ep_moe_block": [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                         ctypes.c_void_p, ctypes.c_void_p],
     "ms_ep_finalize": [ctypes.c_void_p],
+    "ms_rms_norm_fp8": [ctypes.c_char_p, ctypes.c_void_p],
+    "ms_linear_fp8": [ctypes.c_char_p, ctypes.c_void_p],
+    "ms_moe_fp8_workspace": [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)],
+    "ms_moe_fp8_layer": [ctypes.c_char_p, ctypes.c_void_p],
 }
 
 _LIB = None
