@@ -479,6 +479,12 @@ typedef struct ms_fp8_moe {
 int ms_moe_fp8_workspace(const ms_fp8_moe* args, size_t* bytes);
 int ms_moe_fp8_layer(const ms_fp8_moe* args, void* stream);
 
+/* Sticky device-side status of the fp8 operators on `device`: MS_OK, or
+ * MS_E_TIMEOUT when a bounded wait inside one of their kernels ran out (that
+ * call's output is not valid). Also written to *status; reading clears it.
+ * Waits for `stream`; not for use in a capture. */
+int ms_fp8_status(int device, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,8 @@ struct LinearArgs {
   int M, N, K;
 };
 cudaError_t launch_linear_fp8(const LinearArgs& a, int out_dtype, int sms, cudaStream_t s);
+// Address, on the current device, of the status word of the products' kernels.
+cudaError_t linear_fp8_status(int** at);
 
 struct Fp8Matrix {        // [E][n][k] codes
   const uint8_t* q;

@@ -162,3 +162,24 @@ extern "C" int ms_moe_fp8_layer(const ms_fp8_moe* p, void* stream) {
   a.norm_topk = p->norm_topk_prob;
   return launched(me, launch_moe_fp8(a, sm_count(p->device), static_cast<cudaStream_t>(stream)));
 }
+
+extern "C" int ms_fp8_status(int device, int* status, void* stream) {
+  const char* me = "ms_fp8_status";
+  if (!status) return bad(MS_E_INVALID, "%s: status is NULL", me);
+  *status = MS_OK;
+  OnDevice on(device);
+  if (on.err != cudaSuccess) return bad(MS_E_CUDA, "%s: device %d: %s", me, device, cudaGetErrorString(on.err));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int* at = nullptr;
+  if (linear_fp8_status(&at) != cudaSuccess ||
+      cudaMemcpyAsync(status, at, sizeof(int), cudaMemcpyDeviceToHost, s) != cudaSuccess)
+    return bad(MS_E_CUDA, "%s: reading the status failed", me);
+  cudaError_t e = stream_wait_bounded(s);
+  if (e == cudaErrorTimeout)
+    return bad(MS_E_TIMEOUT, "%s: the stream did not finish within the host wait limit (MS_HOST_WAIT_S)", me);
+  if (e != cudaSuccess) return bad(MS_E_CUDA, "%s: %s", me, cudaGetErrorString(e));
+  if (*status == MS_OK) return MS_OK;
+  if (cudaMemsetAsync(at, 0, sizeof(int), s) != cudaSuccess || stream_wait_bounded(s) != cudaSuccess)
+    return bad(MS_E_CUDA, "%s: clearing the status failed", me);
+  return bad(*status, "an fp8 operator's bounded wait ran out: its output is not valid");
+}

@@ -44,6 +44,11 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
+def _stream(device, stream=None):
+    """Raw handle of `stream`, or of the current stream of device `device`."""
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+
+
 def _on_stream(call, stream, device, *args):
     """call(*args) with `stream` current: the tensors it makes belong to the
     stream that writes them."""
@@ -132,7 +137,7 @@ def _norm_call(x, weight, eps, residual, h_out, with_norm):
             0 if h is None else h.data_ptr(), 0 if y is None else y.data_ptr(), q.data_ptr(), s.data_ptr(),
             _row_stride(x2), 0 if res is None else _row_stride(res), d, d, (d + 15) // 16 * 16,
             eps, T, d, _DT[x.dtype], dev)
-        _lib.check(_lib.load().ms_rms_norm_fp8(args, torch._C._cuda_getCurrentRawStream(dev)))
+        _lib.check(_lib.load().ms_rms_norm_fp8(args, _stream(dev)))
     return q, s, (x if h is None else h), y
 
 
@@ -158,6 +163,14 @@ def quantize_fp8(x, stream=None):
     args = (x, None, 0.0, None, None, False)
     q, s, _, _ = _norm_call(*args) if stream is None else _on_stream(_norm_call, stream, x.device.index, *args)
     return q, s
+
+
+def status(device=None, stream=None):
+    """Raise if a bounded wait inside an fp8 kernel on `device` ran out since
+    the last call (its output is not valid). Waits for the stream."""
+    dev = torch.cuda.current_device() if device is None else torch.device(device).index
+    st = ctypes.c_int()
+    _lib.check(_lib.load().ms_fp8_status(dev, ctypes.byref(st), ctypes.c_void_p(_stream(dev, stream))))
 
 
 def quantize_weight_fp8(w):
@@ -255,7 +268,7 @@ class Fp8Linear:
             w, ws, b = self._w
             args = _LINEAR.pack(x.data_ptr(), s.data_ptr(), w, ws, b, out.data_ptr(),
                                 ld, _row_stride(s), self._ld, N, M, N, K, _DT[out_dtype], dev, 0)
-            _lib.check(self._call(args, torch._C._cuda_getCurrentRawStream(dev)))
+            _lib.check(self._call(args, _stream(dev)))
         return out
 
 
@@ -352,5 +365,5 @@ class Fp8MoELayer:
             ws = torch.empty(nb, dtype=torch.uint8, device=dev)
             _lib.check(self._call(
                 self._pack(x2.data_ptr(), 0 if r2 is None else r2.data_ptr(), out.data_ptr(),
-                           ws.data_ptr(), nb, T), torch._C._cuda_getCurrentRawStream(dev.index)))
+                           ws.data_ptr(), nb, T), _stream(dev.index)))
         return out

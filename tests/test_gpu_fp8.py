@@ -7,6 +7,14 @@ from oracle import fp8 as O
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    from moe_stream_b200 import fp8
+    fp8.status()
+
+
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 HALF = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": 2.0 ** -24}
 TINIEST = {"bf16": 2.0 ** -134, "fp16": 2.0 ** -25, "fp32": 2.0 ** -150}   # half a subnormal step
