@@ -87,37 +87,41 @@ __global__ void __launch_bounds__(FEW_THREADS)
   for (int n = 0; n < NT; ++n) acc[n] = 0.f;
 
   if (warp == 4) {
-    if (lane == 0) {
+    if (elect_one())
       for (int b = b0; b < min(b1, b0 + C::STAGES); ++b) tma_prefetch_2d(&tmW, b * 128, n0);
-      grid_wait();
-      for (int b = b0, i = 0; b < b1; ++b, ++i) {
-        const int s = i % C::STAGES;
-        if (i >= C::STAGES && !mbar_wait(&empty[s], ((i / C::STAGES) - 1) & 1, &g_linear_status)) {
-          for (int j = i - C::STAGES; j < i; ++j)      // copies in flight land before the CTA ends
-            mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, &g_linear_status);
-          break;
-        }
+    __syncwarp();
+    grid_wait();
+    for (int b = b0, i = 0; b < b1; ++b, ++i) {
+      const int s = i % C::STAGES;
+      if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, &g_linear_status)) {
+        for (int j = i - C::STAGES; j < i; ++j)      // copies in flight land before the CTA ends
+          mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, &g_linear_status);
+        break;
+      }
+      if (elect_one()) {
         mbar_expect_tx(&full[s], C::STAGE);
         tma_tile_2d(smem + s * C::STAGE, &tmW, b * 128, n0, &full[s]);
         tma_tile_2d(smem + s * C::STAGE + FP8_W_TILE, &tmX, b * 128, m0, &full[s]);
       }
+      __syncwarp();
     }
   } else if (warp == 5) {
     grid_wait();
     grid_release();
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(128, NT);
-      for (int b = b0, i = 0; b < b1; ++b, ++i) {
-        const int s = i % C::STAGES, u = i % C::BUFS;
-        if (!mbar_wait(&full[s], (i / C::STAGES) & 1, &g_linear_status)) break;
-        if (i >= C::BUFS && !mbar_wait(&d_empty[u], ((i / C::BUFS) - 1) & 1, &g_linear_status)) break;
-        tc_after();
+    constexpr uint32_t idesc = idesc_e4m3(128, NT);
+    for (int b = b0, i = 0; b < b1; ++b, ++i) {
+      const int s = i % C::STAGES, u = i % C::BUFS;
+      if (!mbar_wait_step(&full[s], (i / C::STAGES) & 1, &g_linear_status)) break;
+      if (i >= C::BUFS && !mbar_wait_step(&d_empty[u], ((i / C::BUFS) - 1) & 1, &g_linear_status)) break;
+      tc_after();
+      if (elect_one()) {
         const uint64_t ad = k128_desc(smem + s * C::STAGE), bd = k128_desc(smem + s * C::STAGE + FP8_W_TILE);
 #pragma unroll
         for (int j = 0; j < 4; ++j) mma_e4m3(tmem + u * NT, ad + 2 * j, bd + 2 * j, idesc, j != 0);
         mma_done(&empty[s]);
         mma_done(&d_full[u]);
       }
+      __syncwarp();
     }
   } else {
     grid_wait();
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
       named_bar(1, 128);
       for (int c = 0; c < nc; ++c) {
         const int i = c0 - b0 + c, u = i % C::BUFS;
-        if (!mbar_wait(&d_full[u], (i / C::BUFS) & 1, &g_linear_status)) {
+        if (!mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, &g_linear_status)) {
           ok = false;
           break;
         }
@@ -178,12 +182,18 @@ __global__ void __launch_bounds__(FEW_THREADS)
       uint32_t peer[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) peer[r] = r < split ? cluster_map(part, r) : 0;
-      for (int c = rank; c < NT && m0 + c < a.M; c += split) {
-        float v = 0.f;
+      const int cols = min(NT, a.M - m0);
+      for (int c0 = rank; c0 < cols; c0 += 4 * split) {      // four columns' reads in flight
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (r < split) v += ld_cluster_f32(peer[r] + (c * 128 + threadIdx.x) * 4);
-        store_out<OUT>(a.y, (m0 + c) * a.y_stride + n, v + bias);
+          if (r < split)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[j] += ld_cluster_f32(peer[r] + (min(c0 + j * split, cols - 1) * 128 + threadIdx.x) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c0 + j * split < cols) store_out<OUT>(a.y, (m0 + c0 + j * split) * a.y_stride + n, v[j] + bias);
       }
     } else {
 #pragma unroll
@@ -195,9 +205,258 @@ __global__ void __launch_bounds__(FEW_THREADS)
   if (warp == 5) tmem_free(tmem, FEW_TMEM);
 }
 
+// ----------------------------------------------------------------- many rows
+// Rows of x are the MMA's A operand, so a thread that takes a block out of
+// TMEM owns one row and its columns share a scale product. Pairs of CTAs
+// compute 256 x 256 outputs (each CTA loads 128 rows of x and 128 of w per
+// block, half of what a CTA by itself would need for the same tensor work),
+// persistent over the tiles, columns fastest so that the rows of x in flight
+// are few.
+//
+// Every block leaves TMEM, so the round trip (product, barrier, load,
+// barrier to the issuing CTA) has to be hidden: a block is two products of
+// 256 x 128 and TMEM holds four of them; a thread has the last 64 of its 128
+// columns in registers, and gives the buffer back, before it scales them.
+// That takes 232 registers a thread, given by the warps that need none.
+//
+// Warps 0-7 take products out of TMEM and write the outputs (lane quarter
+// warp % 4, column half warp / 4), warp 8 loads, warp 9 of the even CTA
+// issues the MMAs, 10 and 11 bring the scales into shared memory eight blocks
+// at a time (read one block ahead, their latency was the length of a step:
+// 395 us for 16384 x 5120 x 2880). The outputs go through a
+// swizzled 4 KB tile per warp and a tensor store, so that whole lines are
+// written; outputs that a tensor map cannot describe are stored one by one.
+constexpr int PAIR_THREADS = 384, PAIR_STAGES = 5, PAIR_BUFS = 4;
+constexpr int PAIR_STAGE = 2 * FP8_W_TILE;
+constexpr int PAIR_OFF_OUT = PAIR_STAGES * PAIR_STAGE;
+constexpr int PAIR_CHUNK = 8;                 // blocks whose scales are staged together
+constexpr int PAIR_OFF_S = PAIR_OFF_OUT + 8 * 4096;               // [2][CHUNK][128] of x
+constexpr int PAIR_OFF_SW = PAIR_OFF_S + 2 * PAIR_CHUNK * 512;    // [2][CHUNK][2] of w
+constexpr int PAIR_OFF_BAR = PAIR_OFF_SW + 2 * PAIR_CHUNK * 8;
+constexpr int PAIR_SMEM = PAIR_OFF_BAR + 256 + 1024;
+static_assert(PAIR_SMEM <= 232448 && PAIR_SMEM > 232448 - 77824, "alone on its SM");
+
+template <int OUT>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  if (OUT == DT_F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int OUT>
+__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
+    k_linear_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                  const __grid_constant__ CUtensorMap tmY, int y_map, LinearArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_OFF_BAR);
+  uint64_t* full = bars;                     // [STAGES] both CTAs' tiles landed (even CTA's)
+  uint64_t* empty = full + PAIR_STAGES;      // [STAGES] MMAs have read them
+  uint64_t* d_full = empty + PAIR_STAGES;    // [BUFS] a product complete
+  uint64_t* d_empty = d_full + PAIR_BUFS;    // [BUFS] taken out by both CTAs (even CTA's)
+  uint64_t* s_full = d_empty + PAIR_BUFS;    // [2] a chunk's scales staged
+  uint64_t* s_empty = s_full + 2;            // [2] used
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(s_empty + 2);
+  float* s_x = reinterpret_cast<float*>(smem + PAIR_OFF_S);
+  float* s_w = reinterpret_cast<float*>(smem + PAIR_OFF_SW);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
+  const int kb = (a.K + 127) / 128, nt = (a.N + 255) / 256;
+  const int tiles = nt * ((a.M + 255) / 256), step = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < PAIR_STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < PAIR_BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 2), mbar_init(&s_empty[i], 8);
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_map_prefetch(&tmW);
+    tma_map_prefetch(&tmX);
+  }
+  if (warp == 9) tmem_get2(tmem_at, 512);
+  tc_before();
+  cluster_sync();
+  tc_after();
+  const uint32_t tmem = *tmem_at;
+  grid_wait();
+  grid_release();
+
+  if (warp >= 8) {
+    regs_down<40>();
+    if (warp == 8) {
+      const uint32_t full_even = cluster_map(full, 0);
+      bool ok = true;
+      int i = 0;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
+        // half h of the columns: rows n0 + 128 h of w, 64 in each CTA
+        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256 + rank * 64;
+        for (int b = 0; b < kb; ++b, ++i) {
+          const int s = i % PAIR_STAGES;
+          if (i >= PAIR_STAGES && !mbar_wait_step(&empty[s], ((i / PAIR_STAGES) - 1) & 1, &g_linear_status)) {
+            for (int j = i - PAIR_STAGES; j < i && rank == 0; ++j)
+              mbar_wait(&full[j % PAIR_STAGES], (j / PAIR_STAGES) & 1, &g_linear_status);
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * PAIR_STAGE);
+            uint8_t* at = smem + s * PAIR_STAGE;
+            tma_tile_pair(at, &tmX, b * 128, m0, full_even + 8 * s);
+            tma_tile_pair(at + FP8_W_TILE, &tmW, b * 128, n0, full_even + 8 * s);
+            tma_tile_pair(at + FP8_W_TILE + FP8_W_TILE / 2, &tmW, b * 128, n0 + 128, full_even + 8 * s);
+          }
+          __syncwarp();
+        }
+      }
+    } else if (warp == 9 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(256, 128);
+      bool ok = true;
+      int i = 0;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += step)
+        for (int b = 0; b < kb && ok; ++b, ++i) {
+          const int s = i % PAIR_STAGES;
+          ok = mbar_wait_step(&full[s], (i / PAIR_STAGES) & 1, &g_linear_status);
+          const uint64_t ad = k128_desc(smem + s * PAIR_STAGE), bd = k128_desc(smem + s * PAIR_STAGE + FP8_W_TILE);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int u = 2 * (i & 1) + h;
+            if (ok && i >= 2) ok = mbar_wait_step(&d_empty[u], ((i >> 1) - 1) & 1, &g_linear_status);
+            if (!ok) break;
+            tc_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                mma_e4m3_pair(tmem + u * 128, ad + 2 * j, bd + h * (FP8_W_TILE / 2 / 16) + 2 * j, idesc, j != 0);
+              if (h == 1) mma_done_pair(&empty[s]);
+              mma_done_pair(&d_full[u]);
+            }
+            __syncwarp();
+          }
+        }
+    } else if (warp >= 10) {
+      const int r = (warp - 10) * 32 + lane;
+      bool ok = true;
+      int q = 0;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
+        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256;
+        const float* x0 = a.xs + (long long)min(m0 + r, a.M - 1) * a.xs_stride;
+        const float* x1 = a.xs + (long long)min(m0 + r + 64, a.M - 1) * a.xs_stride;
+        // the right half's scales, where the tile has one
+        const float* w = a.ws + (long long)(n0 / 128 + ((lane & 1) && n0 + 128 < a.N ? 1 : 0)) * kb;
+        for (int b0 = 0; b0 < kb; b0 += PAIR_CHUNK, ++q) {
+          float v0[PAIR_CHUNK], v1[PAIR_CHUNK];
+#pragma unroll
+          for (int j = 0; j < PAIR_CHUNK; ++j) {
+            const int b = min(b0 + j, kb - 1);
+            v0[j] = __ldg(x0 + b), v1[j] = __ldg(x1 + b);
+          }
+          const float vw = __ldg(w + min(b0 + ((lane >> 1) & (PAIR_CHUNK - 1)), kb - 1));
+          const int u = q & 1;
+          if (q >= 2 && !mbar_wait_step(&s_empty[u], ((q >> 1) - 1) & 1, &g_linear_status)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int j = 0; j < PAIR_CHUNK; ++j) {
+            s_x[(u * PAIR_CHUNK + j) * 128 + r] = v0[j];
+            s_x[(u * PAIR_CHUNK + j) * 128 + r + 64] = v1[j];
+          }
+          if (warp == 10 && lane < 2 * PAIR_CHUNK) s_w[u * 2 * PAIR_CHUNK + lane] = vw;
+          __syncwarp();
+          if (lane == 0) mbar_arrive1(&s_full[u]);
+        }
+      }
+    }
+  } else {
+    regs_up<232>();
+    const uint32_t d_empty_even = cluster_map(d_empty, 0);
+    const int quarter = warp & 3, half = warp >> 2;
+    uint8_t* out = smem + PAIR_OFF_OUT + warp * 4096;
+    int i = 0, q = 0;
+    bool ok = true;
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
+      const int m = t / nt * 256 + rank * 128 + quarter * 32 + lane, n0 = t % nt * 256 + half * 128;
+      float acc[128];
+#pragma unroll
+      for (int n = 0; n < 128; ++n) acc[n] = 0.f;
+      for (int b = 0; b < kb; ++b, ++i) {
+        const int sb = b % PAIR_CHUNK, su = q & 1, u = 2 * (i & 1) + half;
+        if (sb == 0) ok = mbar_wait_step(&s_full[su], (q >> 1) & 1, &g_linear_status);
+        const float fx = s_x[(su * PAIR_CHUNK + sb) * 128 + quarter * 32 + lane];
+        const uint64_t ff = twice(fx * s_w[(su * PAIR_CHUNK + sb) * 2 + half]);
+        if (!ok || !mbar_wait_step(&d_full[u], (i >> 1) & 1, &g_linear_status)) {
+          ok = false;
+          break;
+        }
+        tc_after();
+        const uint32_t d = tmem + ((uint32_t)(quarter * 32) << 16) + u * 128;
+        uint32_t v[64];
+        tmem_read64(d, v);
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) fma2(acc[j], acc[j + 1], v[j], v[j + 1], ff);
+        tmem_read64(d + 64, v);
+        tc_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_cluster(d_empty_even + 8 * u);
+          if (sb == PAIR_CHUNK - 1 || b == kb - 1) mbar_arrive1(&s_empty[su]);
+        }
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) fma2(acc[64 + j], acc[65 + j], v[j], v[j + 1], ff);
+        if (sb == PAIR_CHUNK - 1 || b == kb - 1) ++q;
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c0 = n0 + 64 * h;
+        if (c0 >= a.N) break;
+        float* v = acc + 64 * h;
+        if (a.bias)
+#pragma unroll
+          for (int n = 0; n < 64; ++n) v[n] += c0 + n < a.N ? __ldg(a.bias + c0 + n) : 0.f;
+        if (y_map) {
+          constexpr int PER = OUT == DT_F32 ? 32 : 64;       // columns of a 128-byte tile row
+#pragma unroll
+          for (int c = 0; c < 64; c += PER) {
+            tma_store_read_wait();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint4 o;
+              if (OUT == DT_F32) {
+                o = make_uint4(__float_as_uint(v[c + 4 * j]), __float_as_uint(v[c + 4 * j + 1]),
+                               __float_as_uint(v[c + 4 * j + 2]), __float_as_uint(v[c + 4 * j + 3]));
+              } else {
+                o.x = pack_out<OUT>(v[8 * j], v[8 * j + 1]);
+                o.y = pack_out<OUT>(v[8 * j + 2], v[8 * j + 3]);
+                o.z = pack_out<OUT>(v[8 * j + 4], v[8 * j + 5]);
+                o.w = pack_out<OUT>(v[8 * j + 6], v[8 * j + 7]);
+              }
+              *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = o;
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && c0 + c < a.N && m < a.M) tma_store_2d(&tmY, out, c0 + c, m);
+          }
+        } else if (m < a.M) {
+#pragma unroll
+          for (int n = 0; n < 64; ++n)
+            if (c0 + n < a.N) store_out<OUT>(a.y, m * a.y_stride + c0 + n, v[n]);
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait();
+  }
+  tc_before();
+  cluster_sync();                            // the even CTA's barriers serve both to the end
+  if (warp == 9) tmem_free2(tmem, 512);
+}
+
 // ------------------------------------------------------------------ launches
-int encode_fp8_map(CUtensorMap* m, const void* base, long long k, long long rows, long long stride, int box_rows,
-                   int mats, long long mat_stride) {
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static const auto fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -206,6 +465,12 @@ int encode_fp8_map(CUtensorMap* m, const void* base, long long k, long long rows
       p = nullptr;
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   }();
+  return fn;
+}
+
+int encode_fp8_map(CUtensorMap* m, const void* base, long long k, long long rows, long long stride, int box_rows,
+                   int mats, long long mat_stride) {
+  const auto fn = encode_fn();
   if (!fn) return -1;
   const cuuint64_t dims[3] = {(cuuint64_t)k, (cuuint64_t)rows, (cuuint64_t)mats};
   const cuuint64_t strides[2] = {(cuuint64_t)stride, (cuuint64_t)mat_stride};
@@ -244,12 +509,56 @@ static cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kern, tw, tx, a);
 }
 
+// y [M][N] as 32-row tiles of 128 bytes, swizzled; false where a tensor map
+// cannot describe it (rows that do not start on 16-byte boundaries)
+template <int OUT>
+static bool encode_out_map(CUtensorMap* m, const LinearArgs& a) {
+  constexpr int SZ = OUT == DT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(a.y) % 16 || a.y_stride * SZ % 16) return false;
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
+  const cuuint64_t strides[1] = {(cuuint64_t)a.y_stride * SZ};
+  const cuuint32_t box[2] = {128 / SZ, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType t = OUT == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : OUT == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(m, t, 2, a.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int OUT>
+static cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t s) {
+  const long long tiles = (long long)((a.N + 255) / 256) * ((a.M + 255) / 256);
+  CUtensorMap tw, tx, ty{};
+  if (encode_fp8_map(&tw, a.w, a.K, a.N, a.w_stride, 64, 0, 0) ||
+      encode_fp8_map(&tx, a.x, a.K, a.M, a.x_stride, 128, 0, 0))
+    return cudaErrorInvalidValue;
+  const int y_map = encode_out_map<OUT>(&ty, a);
+  auto kern = k_linear_pair<OUT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, sms / 2) * 2);
+  cfg.blockDim = dim3(PAIR_THREADS);
+  cfg.dynamicSmemBytes = PAIR_SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, tw, tx, ty, y_map, a);
+}
+
 template <int OUT>
 static cudaError_t launch_out(const LinearArgs& a, int sms, cudaStream_t s) {
   if (a.M <= 16) return launch_few<16, OUT>(a, sms, s);
   if (a.M <= 32) return launch_few<32, OUT>(a, sms, s);
   if (a.M <= 64) return launch_few<64, OUT>(a, sms, s);
-  return launch_few<128, OUT>(a, sms, s);
+  if (a.M <= 256) return launch_few<128, OUT>(a, sms, s);
+  return launch_pair<OUT>(a, sms, s);
 }
 
 cudaError_t launch_linear_fp8(const LinearArgs& a, int out_dtype, int sms, cudaStream_t s) {
