@@ -213,11 +213,12 @@ __global__ void __launch_bounds__(FEW_THREADS)
 // persistent over the tiles, columns fastest so that the rows of x in flight
 // are few.
 //
-// Every block leaves TMEM, so the round trip (product, barrier, load,
-// barrier to the issuing CTA) has to be hidden: a block is two products of
-// 256 x 128 and TMEM holds four of them; a thread has the last 64 of its 128
-// columns in registers, and gives the buffer back, before it scales them.
-// That takes 232 registers a thread, given by the warps that need none.
+// Every block leaves TMEM, so taking one out has to be as fast as the 512
+// cycles of its product: a thread loads 32 columns while it scales the 32
+// before (packed products), across blocks too, and gives the buffer back
+// before the last of them. That takes 232 registers a thread, given by the
+// warps that need none. Two products of 256 x 256 fill TMEM (four of 256 x 128
+// were slower, 266 against 260 us for 16384 x 5120 x 2880: twice the barriers).
 //
 // Warps 0-7 take products out of TMEM and write the outputs (lane quarter
 // warp % 4, column half warp / 4), warp 8 loads, warp 9 of the even CTA
@@ -226,13 +227,14 @@ __global__ void __launch_bounds__(FEW_THREADS)
 // 395 us for 16384 x 5120 x 2880). The outputs go through a
 // swizzled 4 KB tile per warp and a tensor store, so that whole lines are
 // written; outputs that a tensor map cannot describe are stored one by one.
-constexpr int PAIR_THREADS = 384, PAIR_STAGES = 5, PAIR_BUFS = 4;
+constexpr int PAIR_THREADS = 384, PAIR_STAGES = 5, PAIR_BUFS = 2;
 constexpr int PAIR_STAGE = 2 * FP8_W_TILE;
 constexpr int PAIR_OFF_OUT = PAIR_STAGES * PAIR_STAGE;
 constexpr int PAIR_CHUNK = 8;                 // blocks whose scales are staged together
 constexpr int PAIR_OFF_S = PAIR_OFF_OUT + 8 * 4096;               // [2][CHUNK][128] of x
 constexpr int PAIR_OFF_SW = PAIR_OFF_S + 2 * PAIR_CHUNK * 512;    // [2][CHUNK][2] of w
-constexpr int PAIR_OFF_BAR = PAIR_OFF_SW + 2 * PAIR_CHUNK * 8;
+constexpr int PAIR_OFF_B = PAIR_OFF_SW + 2 * PAIR_CHUNK * 8;      // [4][256] bias of a tile
+constexpr int PAIR_OFF_BAR = PAIR_OFF_B + 4 * 1024;
 constexpr int PAIR_SMEM = PAIR_OFF_BAR + 256 + 1024;
 static_assert(PAIR_SMEM <= 232448 && PAIR_SMEM > 232448 - 77824, "alone on its SM");
 
@@ -262,13 +264,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(s_empty + 2);
   float* s_x = reinterpret_cast<float*>(smem + PAIR_OFF_S);
   float* s_w = reinterpret_cast<float*>(smem + PAIR_OFF_SW);
+  float* s_b = reinterpret_cast<float*>(smem + PAIR_OFF_B);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
   const int kb = (a.K + 127) / 128, nt = (a.N + 255) / 256;
   const int tiles = nt * ((a.M + 255) / 256), step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < PAIR_STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < PAIR_BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 8);
+    for (int i = 0; i < PAIR_BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 16);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 2), mbar_init(&s_empty[i], 8);
     fence_barrier_init();
   }
@@ -291,8 +294,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
       bool ok = true;
       int i = 0;
       for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
-        // half h of the columns: rows n0 + 128 h of w, 64 in each CTA
-        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256 + rank * 64;
+        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256 + rank * 128;
         for (int b = 0; b < kb; ++b, ++i) {
           const int s = i % PAIR_STAGES;
           if (i >= PAIR_STAGES && !mbar_wait_step(&empty[s], ((i / PAIR_STAGES) - 1) & 1, &g_linear_status)) {
@@ -306,41 +308,37 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
             uint8_t* at = smem + s * PAIR_STAGE;
             tma_tile_pair(at, &tmX, b * 128, m0, full_even + 8 * s);
             tma_tile_pair(at + FP8_W_TILE, &tmW, b * 128, n0, full_even + 8 * s);
-            tma_tile_pair(at + FP8_W_TILE + FP8_W_TILE / 2, &tmW, b * 128, n0 + 128, full_even + 8 * s);
           }
           __syncwarp();
         }
       }
     } else if (warp == 9 && rank == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(256, 128);
+      constexpr uint32_t idesc = idesc_e4m3(256, 256);
       bool ok = true;
       int i = 0;
       for (int t = blockIdx.x / 2; t < tiles && ok; t += step)
-        for (int b = 0; b < kb && ok; ++b, ++i) {
-          const int s = i % PAIR_STAGES;
-          ok = mbar_wait_step(&full[s], (i / PAIR_STAGES) & 1, &g_linear_status);
-          const uint64_t ad = k128_desc(smem + s * PAIR_STAGE), bd = k128_desc(smem + s * PAIR_STAGE + FP8_W_TILE);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int u = 2 * (i & 1) + h;
-            if (ok && i >= 2) ok = mbar_wait_step(&d_empty[u], ((i >> 1) - 1) & 1, &g_linear_status);
-            if (!ok) break;
-            tc_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                mma_e4m3_pair(tmem + u * 128, ad + 2 * j, bd + h * (FP8_W_TILE / 2 / 16) + 2 * j, idesc, j != 0);
-              if (h == 1) mma_done_pair(&empty[s]);
-              mma_done_pair(&d_full[u]);
-            }
-            __syncwarp();
+        for (int b = 0; b < kb; ++b, ++i) {
+          const int s = i % PAIR_STAGES, u = i & 1;
+          if (!mbar_wait_step(&full[s], (i / PAIR_STAGES) & 1, &g_linear_status) ||
+              (i >= 2 && !mbar_wait_step(&d_empty[u], ((i >> 1) - 1) & 1, &g_linear_status))) {
+            ok = false;
+            break;
           }
+          tc_after();
+          if (elect_one()) {
+            const uint64_t ad = k128_desc(smem + s * PAIR_STAGE), bd = k128_desc(smem + s * PAIR_STAGE + FP8_W_TILE);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_e4m3_pair(tmem + u * 256, ad + 2 * j, bd + 2 * j, idesc, j != 0);
+            mma_done_pair(&d_full[u]);
+            mma_done_pair(&empty[s]);
+          }
+          __syncwarp();
         }
     } else if (warp >= 10) {
       const int r = (warp - 10) * 32 + lane;
       bool ok = true;
-      int q = 0;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
+      int q = 0, tb = 0;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += step, tb = (tb + 1) & 3) {
         const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256;
         const float* x0 = a.xs + (long long)min(m0 + r, a.M - 1) * a.xs_stride;
         const float* x1 = a.xs + (long long)min(m0 + r + 64, a.M - 1) * a.xs_stride;
@@ -365,6 +363,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
             s_x[(u * PAIR_CHUNK + j) * 128 + r + 64] = v1[j];
           }
           if (warp == 10 && lane < 2 * PAIR_CHUNK) s_w[u * 2 * PAIR_CHUNK + lane] = vw;
+          // a tile's bias lies there until its outputs are written: by then this
+          // warp is at most three tiles further
+          if (b0 == 0 && a.bias)
+            for (int n = r; n < 256; n += 64) s_b[tb * 256 + n] = n0 + n < a.N ? __ldg(a.bias + n0 + n) : 0.f;
           __syncwarp();
           if (lane == 0) mbar_arrive1(&s_full[u]);
         }
@@ -375,38 +377,54 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
     const uint32_t d_empty_even = cluster_map(d_empty, 0);
     const int quarter = warp & 3, half = warp >> 2;
     uint8_t* out = smem + PAIR_OFF_OUT + warp * 4096;
-    int i = 0, q = 0;
+    int i = 0, q = 0, tb = 0;
     bool ok = true;
-    for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
+    const uint32_t d0 = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    for (int t = blockIdx.x / 2; t < tiles; t += step, tb = (tb + 1) & 3) {
       const int m = t / nt * 256 + rank * 128 + quarter * 32 + lane, n0 = t % nt * 256 + half * 128;
       float acc[128];
 #pragma unroll
       for (int n = 0; n < 128; ++n) acc[n] = 0.f;
+      uint32_t v0[32], v1[32];
+      ok = mbar_wait_step(&d_full[i & 1], (i >> 1) & 1, &g_linear_status);
+      if (!ok) break;
+      tc_after();
+      tmem_load32(d0 + (i & 1) * 256, v0);
       for (int b = 0; b < kb; ++b, ++i) {
-        const int sb = b % PAIR_CHUNK, su = q & 1, u = 2 * (i & 1) + half;
+        const int sb = b % PAIR_CHUNK, su = q & 1;
+        const bool chunk_end = sb == PAIR_CHUNK - 1 || b == kb - 1;
         if (sb == 0) ok = mbar_wait_step(&s_full[su], (q >> 1) & 1, &g_linear_status);
-        const float fx = s_x[(su * PAIR_CHUNK + sb) * 128 + quarter * 32 + lane];
-        const uint64_t ff = twice(fx * s_w[(su * PAIR_CHUNK + sb) * 2 + half]);
-        if (!ok || !mbar_wait_step(&d_full[u], (i >> 1) & 1, &g_linear_status)) {
-          ok = false;
-          break;
-        }
-        tc_after();
-        const uint32_t d = tmem + ((uint32_t)(quarter * 32) << 16) + u * 128;
-        uint32_t v[64];
-        tmem_read64(d, v);
+        if (!ok) break;
+        const uint64_t ff =
+            twice(s_x[(su * PAIR_CHUNK + sb) * 128 + quarter * 32 + lane] * s_w[(su * PAIR_CHUNK + sb) * 2 + half]);
+        const uint32_t d = d0 + (i & 1) * 256;
+        tmem_wait32(v0);
+        tmem_load32(d + 32, v1);
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) fma2(acc[j], acc[j + 1], v[j], v[j + 1], ff);
-        tmem_read64(d + 64, v);
+        for (int j = 0; j < 32; j += 2) fma2(acc[j], acc[j + 1], v0[j], v0[j + 1], ff);
+        tmem_wait32(v1);
+        tmem_load32(d + 64, v0);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) fma2(acc[32 + j], acc[33 + j], v1[j], v1[j + 1], ff);
+        tmem_wait32(v0);
+        tmem_load32(d + 96, v1);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) fma2(acc[64 + j], acc[65 + j], v0[j], v0[j + 1], ff);
+        tmem_wait32(v1);
         tc_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive_cluster(d_empty_even + 8 * u);
-          if (sb == PAIR_CHUNK - 1 || b == kb - 1) mbar_arrive1(&s_empty[su]);
+          mbar_arrive_cluster(d_empty_even + 8 * (i & 1));
+          if (chunk_end) mbar_arrive1(&s_empty[su]);
+        }
+        q += chunk_end;
+        if (b + 1 < kb) {
+          ok = mbar_wait_step(&d_full[(i + 1) & 1], ((i + 1) >> 1) & 1, &g_linear_status);
+          tc_after();
+          tmem_load32(d0 + ((i + 1) & 1) * 256, v0);
         }
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) fma2(acc[64 + j], acc[65 + j], v[j], v[j + 1], ff);
-        if (sb == PAIR_CHUNK - 1 || b == kb - 1) ++q;
+        for (int j = 0; j < 32; j += 2) fma2(acc[96 + j], acc[97 + j], v1[j], v1[j + 1], ff);
       }
       if (!ok) break;
 #pragma unroll
@@ -414,29 +432,33 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
         const int c0 = n0 + 64 * h;
         if (c0 >= a.N) break;
         float* v = acc + 64 * h;
-        if (a.bias)
+        if (a.bias) {
+          const float4* b4 = reinterpret_cast<const float4*>(s_b + tb * 256 + half * 128 + 64 * h);
 #pragma unroll
-          for (int n = 0; n < 64; ++n) v[n] += c0 + n < a.N ? __ldg(a.bias + c0 + n) : 0.f;
+          for (int n = 0; n < 16; ++n) {
+            const float4 bias = b4[n];
+            v[4 * n] += bias.x, v[4 * n + 1] += bias.y, v[4 * n + 2] += bias.z, v[4 * n + 3] += bias.w;
+          }
+        }
         if (y_map) {
           constexpr int PER = OUT == DT_F32 ? 32 : 64;       // columns of a 128-byte tile row
 #pragma unroll
           for (int c = 0; c < 64; c += PER) {
-            tma_store_read_wait();
-            __syncwarp();
+            uint4 o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              uint4 o;
               if (OUT == DT_F32) {
-                o = make_uint4(__float_as_uint(v[c + 4 * j]), __float_as_uint(v[c + 4 * j + 1]),
-                               __float_as_uint(v[c + 4 * j + 2]), __float_as_uint(v[c + 4 * j + 3]));
+                o[j] = make_uint4(__float_as_uint(v[c + 4 * j]), __float_as_uint(v[c + 4 * j + 1]),
+                                  __float_as_uint(v[c + 4 * j + 2]), __float_as_uint(v[c + 4 * j + 3]));
               } else {
-                o.x = pack_out<OUT>(v[8 * j], v[8 * j + 1]);
-                o.y = pack_out<OUT>(v[8 * j + 2], v[8 * j + 3]);
-                o.z = pack_out<OUT>(v[8 * j + 4], v[8 * j + 5]);
-                o.w = pack_out<OUT>(v[8 * j + 6], v[8 * j + 7]);
+                o[j] = make_uint4(pack_out<OUT>(v[8 * j], v[8 * j + 1]), pack_out<OUT>(v[8 * j + 2], v[8 * j + 3]),
+                                  pack_out<OUT>(v[8 * j + 4], v[8 * j + 5]), pack_out<OUT>(v[8 * j + 6], v[8 * j + 7]));
               }
-              *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = o;
             }
+            tma_store_read_wait();                   // lane 0 sent the tile before
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = o[j];
             fence_async_shared();
             __syncwarp();
             if (lane == 0 && c0 + c < a.N && m < a.M) tma_store_2d(&tmY, out, c0 + c, m);
@@ -532,7 +554,7 @@ template <int OUT>
 static cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t s) {
   const long long tiles = (long long)((a.N + 255) / 256) * ((a.M + 255) / 256);
   CUtensorMap tw, tx, ty{};
-  if (encode_fp8_map(&tw, a.w, a.K, a.N, a.w_stride, 64, 0, 0) ||
+  if (encode_fp8_map(&tw, a.w, a.K, a.N, a.w_stride, 128, 0, 0) ||
       encode_fp8_map(&tx, a.x, a.K, a.M, a.x_stride, 128, 0, 0))
     return cudaErrorInvalidValue;
   const int y_map = encode_out_map<OUT>(&ty, a);

@@ -113,12 +113,20 @@ __device__ __forceinline__ void tmem_wait16(uint32_t* r) {
                : "memory");
 }
 
-// 64 consecutive columns of this thread's lane, here when it returns
-__device__ __forceinline__ void tmem_read64(uint32_t t, uint32_t* r) {
-#pragma unroll
-  for (int i = 0; i < 64; i += 16) tmem_load16(t + i, r + i);
-#pragma unroll
-  for (int i = 0; i < 64; i += 16) tmem_wait16(r + i);
+// 32 consecutive columns; tmem_wait32 before use
+__device__ __forceinline__ void tmem_load32(uint32_t t, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t));
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
+  tmem_wait16(r);
+  tmem_wait16(r + 16);
 }
 // (c0, c1) += (a0, a1) * f, two 32-bit products in one instruction
 __device__ __forceinline__ void fma2(float& c0, float& c1, uint32_t a0, uint32_t a1, uint64_t ff) {
@@ -188,7 +196,7 @@ __device__ __forceinline__ void tma_tile_pair(void* dst, const CUtensorMap* tm, 
       : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // 2-D tile out of shared memory; what lies beyond the matrix is not written
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* src, int x, int y) {
