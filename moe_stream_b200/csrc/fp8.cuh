@@ -86,5 +86,7 @@ struct MoeFp8Args {
 };
 size_t moe_fp8_workspace(int T, int d, int f, int E, int k);
 cudaError_t launch_moe_fp8(const MoeFp8Args& a, int sms, cudaStream_t s);
+// Address, on the current device, of the status word of the layer's kernels.
+cudaError_t moe_fp8_status(int** at);
 
 }  // namespace ms

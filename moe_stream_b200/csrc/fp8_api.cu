@@ -170,16 +170,21 @@ extern "C" int ms_fp8_status(int device, int* status, void* stream) {
   OnDevice on(device);
   if (on.err != cudaSuccess) return bad(MS_E_CUDA, "%s: device %d: %s", me, device, cudaGetErrorString(on.err));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int* at = nullptr;
-  if (linear_fp8_status(&at) != cudaSuccess ||
-      cudaMemcpyAsync(status, at, sizeof(int), cudaMemcpyDeviceToHost, s) != cudaSuccess)
-    return bad(MS_E_CUDA, "%s: reading the status failed", me);
+  int *at[2] = {}, st[2] = {};
+  if (linear_fp8_status(&at[0]) != cudaSuccess || moe_fp8_status(&at[1]) != cudaSuccess)
+    return bad(MS_E_CUDA, "%s: the status words have no address", me);
+  for (int i = 0; i < 2; ++i)
+    if (cudaMemcpyAsync(&st[i], at[i], sizeof(int), cudaMemcpyDeviceToHost, s) != cudaSuccess)
+      return bad(MS_E_CUDA, "%s: reading the status failed", me);
   cudaError_t e = stream_wait_bounded(s);
   if (e == cudaErrorTimeout)
     return bad(MS_E_TIMEOUT, "%s: the stream did not finish within the host wait limit (MS_HOST_WAIT_S)", me);
   if (e != cudaSuccess) return bad(MS_E_CUDA, "%s: %s", me, cudaGetErrorString(e));
+  *status = st[0] ? st[0] : st[1];
   if (*status == MS_OK) return MS_OK;
-  if (cudaMemsetAsync(at, 0, sizeof(int), s) != cudaSuccess || stream_wait_bounded(s) != cudaSuccess)
-    return bad(MS_E_CUDA, "%s: clearing the status failed", me);
+  for (int i = 0; i < 2; ++i)
+    if (cudaMemsetAsync(at[i], 0, sizeof(int), s) != cudaSuccess)
+      return bad(MS_E_CUDA, "%s: clearing the status failed", me);
+  if (stream_wait_bounded(s) != cudaSuccess) return bad(MS_E_CUDA, "%s: clearing the status failed", me);
   return bad(*status, "an fp8 operator's bounded wait ran out: its output is not valid");
 }

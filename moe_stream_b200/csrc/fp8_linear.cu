@@ -37,7 +37,7 @@ __device__ __forceinline__ void store_out(void* y, long long at, float v) {
 // for its cluster.
 constexpr int FEW_THREADS = 192, FEW_TMEM = 256, FEW_CHUNK = 16;
 template <int NT> struct Few {
-  static constexpr int STAGES = NT <= 16 ? 5 : NT <= 64 ? 4 : 3;
+  static constexpr int STAGES = NT <= 16 ? 5 : 4;
   static constexpr int STAGE = FP8_W_TILE + NT * 128;
   static constexpr int BUFS = NT <= 32 ? 8 : FEW_TMEM / NT;
   static constexpr int OFF_S = STAGES * STAGE;                      // scales [FEW_CHUNK][NT]
@@ -225,13 +225,13 @@ __global__ void __launch_bounds__(FEW_THREADS)
 // issues the MMAs, 10 and 11 bring the scales into shared memory eight blocks
 // at a time (read one block ahead, their latency was the length of a step:
 // 395 us for 16384 x 5120 x 2880). The outputs go through a
-// swizzled 4 KB tile per warp and a tensor store, so that whole lines are
+// swizzled 4 KB tile, two per warp, and a tensor store, so that whole lines are
 // written; outputs that a tensor map cannot describe are stored one by one.
-constexpr int PAIR_THREADS = 384, PAIR_STAGES = 5, PAIR_BUFS = 2;
+constexpr int PAIR_THREADS = 384, PAIR_STAGES = 4, PAIR_BUFS = 2;
 constexpr int PAIR_STAGE = 2 * FP8_W_TILE;
 constexpr int PAIR_OFF_OUT = PAIR_STAGES * PAIR_STAGE;
 constexpr int PAIR_CHUNK = 8;                 // blocks whose scales are staged together
-constexpr int PAIR_OFF_S = PAIR_OFF_OUT + 8 * 4096;               // [2][CHUNK][128] of x
+constexpr int PAIR_OFF_S = PAIR_OFF_OUT + 8 * 8192;               // [2][CHUNK][128] of x
 constexpr int PAIR_OFF_SW = PAIR_OFF_S + 2 * PAIR_CHUNK * 512;    // [2][CHUNK][2] of w
 constexpr int PAIR_OFF_B = PAIR_OFF_SW + 2 * PAIR_CHUNK * 8;      // [4][256] bias of a tile
 constexpr int PAIR_OFF_BAR = PAIR_OFF_B + 4 * 1024;
@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
     regs_up<232>();
     const uint32_t d_empty_even = cluster_map(d_empty, 0);
     const int quarter = warp & 3, half = warp >> 2;
-    uint8_t* out = smem + PAIR_OFF_OUT + warp * 4096;
-    int i = 0, q = 0, tb = 0;
+    uint8_t* outs = smem + PAIR_OFF_OUT + warp * 8192;
+    int i = 0, q = 0, tb = 0, ob = 0;
     bool ok = true;
     const uint32_t d0 = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
     for (int t = blockIdx.x / 2; t < tiles; t += step, tb = (tb + 1) & 3) {
@@ -455,8 +455,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
                                   pack_out<OUT>(v[8 * j + 4], v[8 * j + 5]), pack_out<OUT>(v[8 * j + 6], v[8 * j + 7]));
               }
             }
-            tma_store_read_wait();                   // lane 0 sent the tile before
+            tma_store_read_wait();                   // lane 0 sent the tile before the last
             __syncwarp();
+            uint8_t* out = outs + (ob ^= 4096);
 #pragma unroll
             for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = o[j];
             fence_async_shared();
@@ -508,7 +509,13 @@ int encode_fp8_map(CUtensorMap* m, const void* base, long long k, long long rows
 template <int NT, int OUT>
 static cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s) {
   const int tiles = (a.N + 127) / 128, cols = (a.M + NT - 1) / NT, kb = (a.K + 127) / 128;
-  const int split = std::max(1, std::min({8, kb, (sms + tiles * cols - 1) / (tiles * cols)}));
+  // Clusters of 2, 4 and 8 (others fill the GPU unevenly: 23 tiles of K 4096,
+  // 4 CTAs a tile 5.7 us, 6 6.1, 7 6.5). Four CTAs a tile pay while all are
+  // resident, eight only while each has an SM (23 tiles 6.4 us, 40 tiles of K
+  // 2048 9.0 against 5.0; 16 tiles of K 4096 4.7 against 5.2).
+  const long long n = (long long)tiles * cols;
+  int split = 8 * n <= sms ? 8 : 4 * n <= 2 * sms ? 4 : 2 * n <= 2 * sms ? 2 : 1;
+  while (split > kb) split /= 2;
   CUtensorMap tw, tx;
   if (encode_fp8_map(&tw, a.w, a.K, a.N, a.w_stride, 128, 0, 0) ||
       encode_fp8_map(&tx, a.x, a.K, a.M, a.x_stride, NT, 0, 0))
@@ -579,7 +586,13 @@ static cudaError_t launch_out(const LinearArgs& a, int sms, cudaStream_t s) {
   if (a.M <= 16) return launch_few<16, OUT>(a, sms, s);
   if (a.M <= 32) return launch_few<32, OUT>(a, sms, s);
   if (a.M <= 64) return launch_few<64, OUT>(a, sms, s);
-  if (a.M <= 256) return launch_few<128, OUT>(a, sms, s);
+  // Beyond 64 rows the weight is read more than once by the first kernel, and
+  // the second needs tiles for its pairs: the first is ahead while its
+  // 128 x 64 tiles fit the GPU at once (us, first / second: M 128, N 5120, K
+  // 2048 11.9 / 12.0; M 384, N 2880, K 4096 18.2 / 19.7; M 512, N 1024, K 4096
+  // 13.6 / 19.6), behind once they do not (M 256, N 5120, K 2048 15.2 / 12.1;
+  // M 512, N 2880, K 4096 25.7 / 19.8).
+  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) <= sms) return launch_few<64, OUT>(a, sms, s);
   return launch_pair<OUT>(a, sms, s);
 }
 
