@@ -32,11 +32,14 @@
 // Products run on the tensor cores with the weight as operand A (128 rows, the
 // TMEM lanes) and all the tokens (up) or the expert's rows (down) as up to 64
 // columns, so no weight passes through registers. One pipeline serves both: a
-// step is one 128 x 128 weight tile times one activation tile.
-// Warps 0-3 take products out of TMEM and do the rest of a task, warp 4 loads
-// weights and takes tasks, warp 5 issues MMAs, warp 6 loads activations and
-// warp 7 the scales; these two wait for the flags, so that weights are in
-// flight meanwhile.
+// step is two 128 x 128 weight tiles, an up task's gate and up tile of one
+// block or a down task's tiles of two blocks (of one, where the expert has more
+// than 16 rows).
+// Warps 0-3 and 8-11 take products out of TMEM and do the rest of a task, two
+// groups with a task each, so that one's end overlaps the other's products;
+// warp 4 loads weights and takes tasks, warp 5 issues MMAs, warp 6 loads
+// activations and warp 7 the scales; these two wait for the flags, so that
+// weights are in flight meanwhile.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -173,22 +176,25 @@ __global__ void __launch_bounds__(256) k_moe_route(MoeFp8Args a, MoeWs w) {
 }
 
 // ------------------------------------------------------------------- experts
+constexpr int MOE_THREADS = 384, MOE_ROWS = 8;    // rows of activations passed on at a time
 template <int NT> struct Moe {
-  static constexpr int STAGE = FP8_W_TILE + NT * 128;
-  static constexpr int STAGES = NT <= 16 ? 10 : NT <= 32 ? 9 : 7;
-  static constexpr int BUFS = 8;
+  static constexpr int ACT = NT <= 32 ? 4096 : NT * 128;             // activation tiles of a step
+  static constexpr int STAGE = 2 * FP8_W_TILE + ACT;
+  static constexpr int STAGES = NT <= 32 ? 5 : 4;
+  static constexpr int BUFS = NT <= 32 ? 8 : 4;
   static constexpr int OFF_FAC = STAGES * STAGE;                     // [2][FAC][2][NT] scale products
-  static constexpr int OFF_PROB = OFF_FAC + 2 * MOE_FAC * 2 * NT * 4;   // [NT][32]
+  static constexpr int OFF_ROWS = OFF_FAC + 2 * MOE_FAC * 2 * NT * 4;   // [2][2][ROWS][128] gate and up sums
+  static constexpr int OFF_PROB = OFF_ROWS + 2 * 2 * MOE_ROWS * 512; // [NT][32]
   static constexpr int OFF_IND = OFF_PROB + NT * 32 * 4;             // [NT][32] bytes
   static constexpr int OFF_MASK = OFF_IND + NT * 32;                 // [256] tokens of an expert, 64 bits
   static constexpr int OFF_START = OFF_MASK + 256 * 8;               // [256] its first row
   static constexpr int OFF_GROUP = OFF_START + 256 * 4;              // [256] experts that are routed to, ascending
-  static constexpr int OFF_RED = OFF_GROUP + 256;                    // [NT][4] maxima, then four words
-  static constexpr int OFF_TASK = OFF_RED + NT * 16 + 16;            // [4] tasks
-  static constexpr int OFF_BAR = OFF_TASK + 4 * 32;
+  static constexpr int OFF_TASK = OFF_GROUP + 256;                   // [4] tasks
+  static constexpr int OFF_WORD = OFF_TASK + 4 * 32;                 // a few words
+  static constexpr int OFF_BAR = OFF_WORD + 64;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448 && SMEM > 232448 - 77824, "alone on its SM");
-  static_assert(STAGE % 1024 == 0 && BUFS * NT <= 512, "tile alignment, TMEM columns");
+  static_assert(STAGE % 1024 == 0 && BUFS * 2 * NT <= 512, "tile alignment, TMEM columns");
 };
 
 struct __align__(32) Task {
@@ -257,6 +263,19 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(MS_FULL, v, o));
   return v;
 }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(MS_FULL, v, o);
+  return v;
+}
+// a key that orders like the float; a NaN is below all, 0 below every key
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return v != v ? 1u : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 __device__ __forceinline__ float activate(int model, float g, float u) {
   if (model == 1) {
     g = g > 7.f ? 7.f : g;
@@ -264,15 +283,6 @@ __device__ __forceinline__ float activate(int model, float g, float u) {
     return g / (1.f + expf(-1.702f * g)) * (u + 1.f);
   }
   return g / (1.f + expf(-g)) * u;
-}
-// code of feature f of a row whose four warps' maxima are max4; thread 0 the scale
-__device__ __forceinline__ void put_code(const MoeWs& w, int f_all, int f, int tid, int tile, int tiles, long long row,
-                                         float h, const float* max4) {
-  const float4 m = *reinterpret_cast<const float4*>(max4);
-  float inv;
-  const float s = group_scale(max_nan(max_nan(m.x, m.y), max_nan(m.z, m.w)), &inv);
-  if (f < f_all) w.hq[row * f_all + f] = (uint8_t)e4m3x2(h * inv, 0.f);
-  if (tid == 0) w.hs[row * tiles + tile] = s;
 }
 __device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
@@ -293,7 +303,7 @@ struct MoeMaps {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(MOE_THREADS, 1)
     k_moe_experts(const __grid_constant__ MoeMaps maps, const __grid_constant__ MoeFp8Args a,
                   const __grid_constant__ MoeWs w) {
   using C = Moe<NT>;
@@ -305,8 +315,7 @@ __global__ void __launch_bounds__(256, 1)
   unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::OFF_MASK);
   int* s_start = reinterpret_cast<int*>(smem + C::OFF_START);
   uint8_t* s_group = smem + C::OFF_GROUP;
-  float* s_red = reinterpret_cast<float*>(smem + C::OFF_RED);
-  volatile int* s_word = reinterpret_cast<volatile int*>(s_red + NT * 4); // last, groups, S1, S2
+  volatile int* s_word = reinterpret_cast<volatile int*>(smem + C::OFF_WORD);   // last [2], groups, S1, S2
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);        // [STAGES] both tiles landed
   uint64_t* empty = full + C::STAGES;                                     // [STAGES] read by the MMAs
   uint64_t* d_full = empty + C::STAGES;                                   // [BUFS] a product complete
@@ -325,10 +334,10 @@ __global__ void __launch_bounds__(256, 1)
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
     for (int i = 0; i < C::BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4);
     for (int i = 0; i < 2; ++i) mbar_init(&f_full[i], 1), mbar_init(&f_empty[i], 4);
-    for (int i = 0; i < 4; ++i) mbar_init(&t_full[i], 1), mbar_init(&t_empty[i], 7);
+    for (int i = 0; i < 4; ++i) mbar_init(&t_full[i], 1), mbar_init(&t_empty[i], 11);
     fence_barrier_init();
   }
-  for (int e = threadIdx.x; e < 256; e += 256) s_mask[e] = 0;
+  if (threadIdx.x < 256) s_mask[threadIdx.x] = 0;
   if (warp == 5) tmem_get(tmem_at, 512);
   if (warp == 4 && lane < 6) tma_map_prefetch(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
   tc_before();
@@ -340,91 +349,136 @@ __global__ void __launch_bounds__(256, 1)
   unsigned first_task = 0;
   if (warp == 4 && lane == 0) first_task = atomicAdd(w.next, 1u);    // back by the time it can be read
 
-  // ---- the routing, a warp per token
-  for (int t = warp; t < a.T; t += 8) {
-    uint32_t key[8];                        // ordered like the logits; a NaN is below all
-    float v[8];
-    bool nan = false;
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = lane + 32 * i;
-      v[i] = e < a.E ? __ldcg(w.logits + t * a.E + e) + 0.f : 0.f;       // -0 is 0
+  // ---- the routing
+  if (a.T <= 4) {
+    // few tokens: a thread per expert counts the logits above its own
+    uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + C::OFF_ROWS);
+    uint32_t* s_top = s_key + 256;
+    for (int t = 0; t < a.T; ++t) {
+      const int e = threadIdx.x;
+      const bool in = e < a.E;
+      const float v = in ? __ldcg(w.logits + t * a.E + e) + 0.f : 0.f;         // -0 is 0
+      const uint32_t key = in ? order_key(v) : 0u;
+      if (e < 256) s_key[e] = key;
+      const bool nan = __syncthreads_or(v != v);
+      if (in) {
+        int rank = 0;
+        for (int q = 0; q < a.E; q += 4) {
+          const uint4 o = *reinterpret_cast<const uint4*>(s_key + q);
+          rank += o.x > key || (o.x == key && q < e);
+          rank += o.y > key || (o.y == key && q + 1 < e);
+          rank += o.z > key || (o.z == key && q + 2 < e);
+          rank += o.w > key || (o.w == key && q + 3 < e);
+        }
+        if (rank < a.k) {
+          s_ind[t * 32 + rank] = (uint8_t)e;
+          s_top[rank] = key;
+          atomicOr(&s_mask[e], 1ull << t);
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const float m = nan ? __uint_as_float(0x7fc00000u) : key_value(s_top[0]);
+        const float p = lane < a.k ? expf(key_value(s_top[lane]) - m) : 0.f;
+        float sum = p;
+        if (a.model == 0 && !a.norm_topk) {
+          sum = 0.f;
+          for (int q = lane; q < a.E; q += 32) sum += expf(key_value(s_key[q]) - m);
+        }
+        sum = warp_sum(sum);
+        if (lane < a.k) s_prob[t * 32 + lane] = p / sum;
+      }
+      if (t + 1 < a.T) __syncthreads();
     }
+  } else {
+    // a warp per token, the largest one after another
+    for (int t = warp; t < a.T; t += MOE_THREADS / 32) {
+      uint32_t key[8];
+      float v[8];
+      bool nan = false;
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t b = __float_as_uint(v[i]);
-      nan |= v[i] != v[i];
-      key[i] = lane + 32 * i < a.E ? (v[i] != v[i] ? 1u : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u)) : 0u;
-      top = max(top, key[i]);
-    }
-    top = __reduce_max_sync(MS_FULL, top);
-    const uint32_t top_bits = top & 0x80000000u ? top ^ 0x80000000u : ~top;
-    const float m = __any_sync(MS_FULL, nan) ? __uint_as_float(0x7fc00000u) : __uint_as_float(top_bits);
-    uint32_t mine_key = 0;                  // lane j: the j-th choice
-    int mine = 0;
-    float all = 0.f;
-    if (a.model == 0 && !a.norm_topk) {
+      for (int i = 0; i < 8; ++i) {
+        const int e = lane + 32 * i;
+        v[i] = e < a.E ? __ldcg(w.logits + t * a.E + e) + 0.f : 0.f;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) all += lane + 32 * i < a.E ? expf(v[i] - m) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        nan |= v[i] != v[i];
+        key[i] = lane + 32 * i < a.E ? order_key(v[i]) : 0u;
+        top = max(top, key[i]);
+      }
+      const float m0 = key_value(__reduce_max_sync(MS_FULL, top));
+      const float m = __any_sync(MS_FULL, nan) ? __uint_as_float(0x7fc00000u) : m0;
+      uint32_t mine_key = 0;                  // lane j: the j-th choice
+      int mine = 0;
+      float all = 0.f;
+      if (a.model == 0 && !a.norm_topk) {
 #pragma unroll
-      for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(MS_FULL, all, o);
-    }
-    for (int j = 0; j < a.k; ++j) {
-      const uint32_t b0 = max(max(key[0], key[1]), max(key[2], key[3]));
-      const uint32_t b1 = max(max(key[4], key[5]), max(key[6], key[7]));
-      const uint32_t best = __reduce_max_sync(MS_FULL, max(b0, b1));
-      int e = 1 << 20;
+        for (int i = 0; i < 8; ++i) all += lane + 32 * i < a.E ? expf(v[i] - m) : 0.f;
+        all = warp_sum(all);
+      }
+      for (int j = 0; j < a.k; ++j) {
+        const uint32_t b0 = max(max(key[0], key[1]), max(key[2], key[3]));
+        const uint32_t b1 = max(max(key[4], key[5]), max(key[6], key[7]));
+        const uint32_t best = __reduce_max_sync(MS_FULL, max(b0, b1));
+        int e = 1 << 20;
 #pragma unroll
-      for (int i = 7; i >= 0; --i)
-        if (key[i] == best) e = lane + 32 * i;
-      const int first = __reduce_min_sync(MS_FULL, e);
+        for (int i = 7; i >= 0; --i)
+          if (key[i] == best) e = lane + 32 * i;
+        const int first = __reduce_min_sync(MS_FULL, e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i == first) key[i] = 0;
-      if (lane == j) mine = first, mine_key = best;
-    }
-    const float l = __uint_as_float(mine_key & 0x80000000u ? mine_key ^ 0x80000000u : ~mine_key);
-    float p = lane < a.k ? expf(l - m) : 0.f, sel = p;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sel += __shfl_xor_sync(MS_FULL, sel, o);
-    if (lane < a.k) {
-      s_prob[t * 32 + lane] = p / (a.model == 1 || a.norm_topk ? sel : all);
-      s_ind[t * 32 + lane] = (uint8_t)mine;
-      atomicOr(&s_mask[mine], 1ull << t);
+        for (int i = 0; i < 8; ++i)
+          if (lane + 32 * i == first) key[i] = 0;
+        if (lane == j) mine = first, mine_key = best;
+      }
+      const float p = lane < a.k ? expf(key_value(mine_key) - m) : 0.f;
+      const float sel = warp_sum(p);
+      if (lane < a.k) {
+        s_prob[t * 32 + lane] = p / (a.model == 1 || a.norm_topk ? sel : all);
+        s_ind[t * 32 + lane] = (uint8_t)mine;
+        atomicOr(&s_mask[mine], 1ull << t);
+      }
     }
   }
   __syncthreads();
-  if (warp == 0) {                          // groups in expert order and their first rows
-    int G = 0, row = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 32) {
-      const int e = e0 + lane, n = e < a.E ? __popcll(s_mask[e]) : 0;
-      const unsigned has = __ballot_sync(MS_FULL, n > 0);
-      if (!has) continue;
-      int at = n;
+  if (warp == 0) {                          // groups in expert order and their first rows, eight experts a lane
+    int n[8], sum = 0;                      // rows in the low half, groups in the high
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(MS_FULL, at, o);
-        if (lane >= o) at += u;
-      }
-      if (n > 0) {
-        s_group[G + __popc(has & ((1u << lane) - 1))] = (uint8_t)e;
-        s_start[e] = row + at - n;
-      }
-      G += __popc(has);
-      row += __shfl_sync(MS_FULL, at, 31);
+    for (int i = 0; i < 8; ++i) {
+      n[i] = __popcll(s_mask[lane * 8 + i]);
+      sum += n[i] + (n[i] ? 1 << 16 : 0);
     }
+    int at = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(MS_FULL, at, o);
+      if (lane >= o) at += u;
+    }
+    const int G = __shfl_sync(MS_FULL, at, 31) >> 16;
+    at -= sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n[i]) {
+        s_group[at >> 16] = (uint8_t)(lane * 8 + i);
+        s_start[lane * 8 + i] = at & 0xffff;
+        at += n[i] + (1 << 16);
+      }
     const int s1 = choose_split(G * blocks128(a.f), blocks128(a.d), gridDim.x, w.cap1, 2.f);
     const int s2 = choose_split(G * blocks128(a.d), blocks128(a.f), gridDim.x, w.cap2, 0.5f);
-    if (lane == 0) s_word[1] = G, s_word[2] = s1, s_word[3] = s2;
+    if (lane == 0) s_word[2] = G, s_word[3] = s1, s_word[4] = s2;
   }
   __syncthreads();
   Shape sh;
-  sh.G = s_word[1], sh.S1 = s_word[2], sh.S2 = s_word[3];
+  sh.G = s_word[2], sh.S1 = s_word[3], sh.S2 = s_word[4];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
   sh.n_up = sh.G * sh.FT * sh.S1, sh.n_dn = sh.G * sh.DT * sh.S2;
   sh.n_co = sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
 
+  // blocks of a down step
+  auto down_per = [&](int g) { return __popcll(s_mask[s_group[g]]) <= 16 ? 2 : 1; };
+
+  if (NT == 64 && warp >= 4 && warp < 8) regs_down<40>();
   if (warp == 4) {
     // ---- tasks and weight tiles
     bool ok = true;
@@ -444,24 +498,29 @@ __global__ void __launch_bounds__(256, 1)
         ok = mbar_wait_step(&t_empty[n & 3], (n >> 2) & 1, status);
         continue;
       }
-      const int e = s_group[t.g];
-      const int per = t.kind == 0 ? 2 : 1;
-      for (int b = t.b0; b < t.b1 && ok; ++b)
-        for (int h = 0; h < per; ++h, ++i) {
-          const int s = i % C::STAGES;
-          if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
-            // copies in flight land before the CTA ends
-            for (int j = i - C::STAGES; j < i && mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, status);) ++j;
-            ok = false;
-            break;
-          }
-          if (elect_one()) {
-            mbar_expect_tx(&full[s], FP8_W_TILE);
-            tma_tile_3d(smem + s * C::STAGE, t.kind == 1 ? &maps.down : h ? &maps.up : &maps.gate, b * 128,
-                        t.tile * 128, e, &full[s]);
-          }
-          __syncwarp();
+      const int e = s_group[t.g], per = t.kind == 0 ? 1 : down_per(t.g);
+      for (int b = t.b0; b < t.b1; b += per, ++i) {
+        const int s = i % C::STAGES;
+        if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
+          // copies in flight land before the CTA ends
+          for (int j = i - C::STAGES; j < i && mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, status);) ++j;
+          ok = false;
+          break;
         }
+        if (elect_one()) {
+          uint8_t* at = smem + s * C::STAGE;
+          const int tiles = t.kind == 0 ? 2 : min(per, t.b1 - b);
+          mbar_expect_tx(&full[s], tiles * FP8_W_TILE);
+          if (t.kind == 0) {
+            tma_tile_3d(at, &maps.gate, b * 128, t.tile * 128, e, &full[s]);
+            tma_tile_3d(at + FP8_W_TILE, &maps.up, b * 128, t.tile * 128, e, &full[s]);
+          } else {
+            for (int h = 0; h < tiles; ++h)
+              tma_tile_3d(at + h * FP8_W_TILE, &maps.down, (b + h) * 128, t.tile * 128, e, &full[s]);
+          }
+        }
+        __syncwarp();
+      }
     }
   } else if (warp == 5) {
     // ---- MMAs
@@ -474,10 +533,9 @@ __global__ void __launch_bounds__(256, 1)
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
       if (t.kind == 3) break;
       if (t.kind == 2) continue;
-      const bool few = NT > 16 && t.kind == 1 && __popcll(s_mask[s_group[t.g]]) <= 16;
-      const uint32_t idesc = few ? idesc_e4m3(128, 16) : idesc_e4m3(128, NT);
-      const int steps = (t.b1 - t.b0) * (t.kind == 0 ? 2 : 1);
-      for (int j = 0; j < steps; ++j, ++i) {
+      const int per = t.kind == 0 ? 1 : down_per(t.g);
+      const uint32_t idesc = t.kind == 1 && per == 2 ? idesc_e4m3(128, 16) : idesc_e4m3(128, NT);
+      for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int s = i % C::STAGES, u = i % C::BUFS;
         if (!mbar_wait_step(&full[s], (i / C::STAGES) & 1, status) ||
             (i >= C::BUFS && !mbar_wait_step(&d_empty[u], ((i / C::BUFS) - 1) & 1, status))) {
@@ -486,11 +544,16 @@ __global__ void __launch_bounds__(256, 1)
         }
         tc_after();
         if (elect_one()) {
-          const uint64_t ad = k128_desc(smem + s * C::STAGE), bd = k128_desc(smem + s * C::STAGE + FP8_W_TILE);
+          const uint8_t* at = smem + s * C::STAGE;
+          const uint64_t ad = k128_desc(at), bd = k128_desc(at + 2 * FP8_W_TILE);
+          const int tiles = t.kind == 0 ? 2 : min(per, t.b1 - b);
+          const int next_b = t.kind == 0 ? 0 : 2048 / 16;
+          for (int h = 0; h < tiles; ++h)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mma_e4m3(tmem + u * NT, ad + 2 * q, bd + 2 * q, idesc, q != 0);
-          mma_done(&empty[s]);
+            for (int q = 0; q < 4; ++q)
+              mma_e4m3(tmem + (2 * u + h) * NT, ad + h * (FP8_W_TILE / 16) + 2 * q, bd + h * next_b + 2 * q, idesc, q != 0);
           mma_done(&d_full[u]);
+          mma_done(&empty[s]);
         }
         __syncwarp();
       }
@@ -506,25 +569,31 @@ __global__ void __launch_bounds__(256, 1)
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
       if (t.kind == 3) break;
       if (t.kind == 2) continue;
-      const int e = s_group[t.g], rows = __popcll(s_mask[e]), start = s_start[e], nb = t.b1 - t.b0;
+      const int start = s_start[s_group[t.g]], per = t.kind == 0 ? 1 : down_per(t.g);
       if (t.kind == 1) {
         for (int b = t.b0 + lane; b < t.b1; b += 32) wait_count(w.flag + t.g * sh.FT + b, 1);
         __syncwarp();
         fence_async_all();
       }
-      const bool few = NT > 16 && t.kind == 1 && rows <= 16;
-      const int steps = nb * (t.kind == 0 ? 2 : 1);
-      for (int j = 0; j < steps; ++j, ++i) {
+      for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int s = i % C::STAGES;
         if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
           ok = false;
           break;
         }
-        const int b = t.b0 + (t.kind == 0 ? j >> 1 : j);
         if (elect_one()) {
-          mbar_expect_tx(&full[s], few ? 16 * 128 : NT * 128);
-          tma_tile_2d(smem + s * C::STAGE + FP8_W_TILE, t.kind == 0 ? &maps.x : few ? &maps.h16 : &maps.h, b * 128,
-                      t.kind == 0 ? 0 : start, &full[s]);
+          uint8_t* at = smem + s * C::STAGE + 2 * FP8_W_TILE;
+          if (t.kind == 0) {
+            mbar_expect_tx(&full[s], NT * 128);
+            tma_tile_2d(at, &maps.x, b * 128, 0, &full[s]);
+          } else if (per == 1) {
+            mbar_expect_tx(&full[s], NT * 128);
+            tma_tile_2d(at, &maps.h, b * 128, start, &full[s]);
+          } else {
+            const int tiles = min(2, t.b1 - b);
+            mbar_expect_tx(&full[s], tiles * 2048);
+            for (int h = 0; h < tiles; ++h) tma_tile_2d(at + h * 2048, &maps.h16, (b + h) * 128, start, &full[s]);
+          }
         }
         __syncwarp();
       }
@@ -569,24 +638,28 @@ __global__ void __launch_bounds__(256, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive1(&f_full[u]);
     }
-  } else if (warp < 4) {
+  } else {
     // ---- products out of TMEM, and what follows them
+    if (NT == 64) regs_up<232>();
+    const int grp = warp >> 3, tid = threadIdx.x & 127, bar = 1 + grp;
     bool ok = true;
     int i = 0, c = 0;
-    const int tid = threadIdx.x;
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    float* s_rows = reinterpret_cast<float*>(smem + C::OFF_ROWS) + grp * (2 * MOE_ROWS * 128);
     float acc[2][NT];
     for (int n = 0; ok; ++n) {
       if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
       const Task t = s_task[n & 3];
       __syncwarp();
-      if (t.kind != 2 && lane == 0) mbar_arrive1(&t_empty[n & 3]);
+      const bool combine = t.kind == 2 && grp == 0;
+      if (!combine && lane == 0) mbar_arrive1(&t_empty[n & 3]);
       if (t.kind == 3) break;
       if (t.kind == 2) {
+        if (!combine) continue;
         // y of four tokens, one per warp: rows in the order of the token's
         // choices, ranges in order
         if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2));
-        named_bar(1, 128);
+        named_bar(bar, 128);
         const int f = t.tile * 128 + lane * 4, tok = t.s * COMBINE_T + warp;
         if (f < a.d && tok < a.T) {
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -632,23 +705,26 @@ __global__ void __launch_bounds__(256, 1)
         if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
         continue;
       }
+      const int per = t.kind == 0 ? 1 : down_per(t.g);
+      if ((c & 1) != grp) {                  // the other group's
+        i += (t.b1 - t.b0 + per - 1) / per;
+        ++c;
+        continue;
+      }
       const int e = s_group[t.g], start = s_start[e];
       const unsigned long long mask = s_mask[e];
       const int rows = __popcll(mask);
       const int cols = t.kind == 0 ? a.T : rows;
-      const float* fac = s_fac + (c & 1) * (MOE_FAC * 2 * NT);
-      ok = mbar_wait_step(&f_full[c & 1], (c >> 1) & 1, status);
+      const float* fac = s_fac + grp * (MOE_FAC * 2 * NT);
+      ok = mbar_wait_step(&f_full[grp], (c >> 1) & 1, status);
 #pragma unroll
       for (int m = 0; m < NT; ++m) acc[0][m] = acc[1][m] = 0.f;
-      auto take = [&](float* sum, const float* f) {
-        const int u = i % C::BUFS;
-        if (!mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, status)) return false;
-        tc_after();
+      auto take = [&](float* sum, uint32_t at, const float* f) {
 #pragma unroll
         for (int m = 0; m < NT; m += 16) {
           if (m >= cols) break;
           uint32_t v[16];
-          tmem_load16(lanes + u * NT + m, v);
+          tmem_load16(at + m, v);
           tmem_wait16(v);
           const float4* f4 = reinterpret_cast<const float4*>(f + m);
 #pragma unroll
@@ -660,19 +736,25 @@ __global__ void __launch_bounds__(256, 1)
             sum[m + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), x.w, sum[m + 4 * q + 3]);
           }
         }
+      };
+      for (int b = t.b0; b < t.b1; b += per, ++i) {
+        const int u = i % C::BUFS;
+        if (!ok || !mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, status)) {
+          ok = false;
+          break;
+        }
+        tc_after();
+        const float* f = fac + (b - t.b0) * 2 * NT;
+        const uint32_t at = lanes + 2 * u * NT;
+        take(acc[0], at, f);
+        if (t.kind == 0) take(acc[1], at + NT, f + NT);
+        else if (per == 2 && b + 1 < t.b1) take(acc[0], at + NT, f + 2 * NT);
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive1(&d_empty[u]);
-        ++i;
-        return true;
-      };
-      for (int b = t.b0; b < t.b1 && ok; ++b) {
-        const float* f = fac + (b - t.b0) * 2 * NT;
-        ok = take(acc[0], f);
-        if (t.kind == 0 && ok) ok = take(acc[1], f + NT);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive1(&f_empty[c & 1]);
+      if (lane == 0) mbar_arrive1(&f_empty[grp]);
       ++c;
       if (!ok) break;
       const int f = t.tile * 128 + tid;
@@ -682,13 +764,11 @@ __global__ void __launch_bounds__(256, 1)
 #pragma unroll
           for (int m = 0; m < NT; ++m)
             if (m < rows) __stcg(part + (long long)m * a.d, acc[0][m]);
-        named_bar(1, 128);
+        named_bar(bar, 128);
         if (tid == 0) red_release(w.dn_done + t.tile);
         continue;
       }
       const int tile = t.g * sh.FT + t.tile;
-      const float bg = a.gate.bias && f < a.f ? __ldg(a.gate.bias + (long long)e * a.f + f) : 0.f;
-      const float bu = a.up.bias && f < a.f ? __ldg(a.up.bias + (long long)e * a.f + f) : 0.f;
       if (sh.S1 > 1) {
         if (f < a.f) {
           float* pg = w.up_part + (t.s * 2ll * P + start) * a.f + f;
@@ -702,53 +782,68 @@ __global__ void __launch_bounds__(256, 1)
               at += a.f;
             }
         }
-        named_bar(1, 128);
-        if (tid == 0) s_word[0] = add_acq_rel(w.brought + tile) == (unsigned)(sh.S1 - 1);
-        named_bar(1, 128);
-        const bool last = s_word[0];
-        named_bar(1, 128);                   // all have read the word
+        named_bar(bar, 128);
+        if (tid == 0) s_word[grp] = add_acq_rel(w.brought + tile) == (unsigned)(sh.S1 - 1);
+        named_bar(bar, 128);
+        const bool last = s_word[grp];
+        named_bar(bar, 128);                 // all have read the word
         if (!last) continue;
-        for (int r0 = 0; r0 < rows; r0 += 4) {
-          float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-          if (f < a.f)
-#pragma unroll 3
-            for (int s = 0; s < sh.S1; ++s)
+      }
+      // a warp per row: four features a lane
+      const int f4 = t.tile * 128 + lane * 4;
+      const bool in = f4 < a.f;
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (in)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float* at = w.up_part + (s * 2ll * P + start + min(r0 + r, rows - 1)) * a.f + f;
-                g[r] += __ldcg(at), u[r] += __ldcg(at + (long long)P * a.f);
-              }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            g[r] = f < a.f ? activate(a.model, g[r] + bg, u[r] + bu) : 0.f;
-            u[r] = warp_max(fabsf(g[r]));
-          }
-          if (lane == 0)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s_red[r * 4 + warp] = u[r];
-          named_bar(1, 128);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r0 + r < rows) put_code(w, a.f, f, tid, t.tile, sh.KB2, start + r0 + r, g[r], s_red + r * 4);
-          named_bar(1, 128);                 // the maxima have been read
+        for (int q = 0; q < 4; ++q) {
+          if (a.gate.bias) bg[q] = __ldg(a.gate.bias + (long long)e * a.f + f4 + q);
+          if (a.up.bias) bu[q] = __ldg(a.up.bias + (long long)e * a.f + f4 + q);
         }
-      } else {
-        // a row's activations stay in the registers of its column
+      for (int r0 = 0; r0 < rows; r0 += MOE_ROWS) {
+        if (sh.S1 == 1) {                    // this tile's sums are in the registers of their columns
+          int r = 0;
 #pragma unroll
-        for (int m = 0; m < NT; ++m)
-          if (mask >> m & 1) {
-            acc[0][m] = f < a.f ? activate(a.model, acc[0][m] + bg, acc[1][m] + bu) : 0.f;
-            const float top = warp_max(fabsf(acc[0][m]));
-            if (lane == 0) s_red[m * 4 + warp] = top;
+          for (int m = 0; m < NT; ++m)
+            if (mask >> m & 1) {
+              if (r >= r0 && r < r0 + MOE_ROWS) {
+                s_rows[(r - r0) * 128 + tid] = acc[0][m];
+                s_rows[(MOE_ROWS + r - r0) * 128 + tid] = acc[1][m];
+              }
+              ++r;
+            }
+          named_bar(bar, 128);
+        }
+        for (int r = r0 + (warp & 3); r < min(rows, r0 + MOE_ROWS); r += 4) {
+          float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+          if (sh.S1 == 1) {
+            g = *reinterpret_cast<const float4*>(s_rows + (r - r0) * 128 + lane * 4);
+            u = *reinterpret_cast<const float4*>(s_rows + (MOE_ROWS + r - r0) * 128 + lane * 4);
+          } else if (in) {
+            const float* at = w.up_part + (long long)(start + r) * a.f + f4;
+#pragma unroll 4
+            for (int s = 0; s < sh.S1; ++s) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(at + s * 2ll * P * a.f));
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(at + (s * 2ll + 1) * P * a.f));
+              g.x += x.x, g.y += x.y, g.z += x.z, g.w += x.w;
+              u.x += y.x, u.y += y.y, u.z += y.z, u.w += y.w;
+            }
           }
-        named_bar(1, 128);
-        int row = start;
-#pragma unroll
-        for (int m = 0; m < NT; ++m)
-          if (mask >> m & 1) put_code(w, a.f, f, tid, t.tile, sh.KB2, row++, acc[0][m], s_red + m * 4);
+          const float h0 = in ? activate(a.model, g.x + bg[0], u.x + bu[0]) : 0.f;
+          const float h1 = in ? activate(a.model, g.y + bg[1], u.y + bu[1]) : 0.f;
+          const float h2 = in ? activate(a.model, g.z + bg[2], u.z + bu[2]) : 0.f;
+          const float h3 = in ? activate(a.model, g.w + bg[3], u.w + bu[3]) : 0.f;
+          float inv;
+          const float s = group_scale(
+              warp_max(max_nan(max_nan(fabsf(h0), fabsf(h1)), max_nan(fabsf(h2), fabsf(h3)))), &inv);
+          if (in)
+            *reinterpret_cast<uint32_t*>(w.hq + (long long)(start + r) * a.f + f4) =
+                e4m3x2(h0 * inv, h1 * inv) | e4m3x2(h2 * inv, h3 * inv) << 16;
+          if (lane == 0) w.hs[(long long)(start + r) * sh.KB2 + t.tile] = s;
+        }
+        if (sh.S1 == 1) named_bar(bar, 128); // the rows have been read
       }
       fence_async_all();                     // the codes are read by tensor copies
-      named_bar(1, 128);
+      named_bar(bar, 128);
       if (tid == 0) red_release(w.flag + tile);
     }
   }
@@ -778,7 +873,7 @@ static cudaError_t launch_experts(const MoeFp8Args& a, const MoeWs& w, int sms, 
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(MOE_THREADS);
   cfg.dynamicSmemBytes = Moe<NT>::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
