@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(FEW_THREADS)
     grid_wait();
     const float* ws = a.ws + (long long)blockIdx.y * kb;
     bool ok = true;
-    for (int c0 = b0; c0 < b1 && ok; c0 += FEW_CHUNK) {
+    // after a wait that ran out the warp goes on to the barriers, without the
+    // products: others may be waiting there
+    for (int c0 = b0; c0 < b1; c0 += FEW_CHUNK) {
       const int nc = min(FEW_CHUNK, b1 - c0);
       named_bar(1, 128);                     // the chunk before has been used
       for (int i = threadIdx.x; i < nc * NT; i += 128) {
@@ -137,10 +139,8 @@ __global__ void __launch_bounds__(FEW_THREADS)
       named_bar(1, 128);
       for (int c = 0; c < nc; ++c) {
         const int i = c0 - b0 + c, u = i % C::BUFS;
-        if (!mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, &g_linear_status)) {
-          ok = false;
-          break;
-        }
+        ok = ok && mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, &g_linear_status);
+        if (!ok) break;
         tc_after();
         const uint32_t t = tmem + ((uint32_t)(warp * 32) << 16) + u * NT;
 #pragma unroll

@@ -12,8 +12,9 @@
 //
 // Bound by memory: every routed expert's codes once. k_moe_route makes the
 // logits and x's codes; k_moe_experts streams the experts. Each of its CTAs
-// (one per SM) works out the routing for itself, which is less than a trip
-// through memory, then takes tasks off one counter:
+// (one per SM) works out the routing of up to four tokens for itself, which is
+// less than a trip through memory; more tokens are shared out. Then it takes
+// tasks off one counter:
 //
 //   up       128 features of d_ff of one expert, gate and up rows, a range of
 //            the blocks of d (all of them where there are tiles enough; else
@@ -30,11 +31,11 @@
 // results do not depend on timing.
 //
 // Products run on the tensor cores with the weight as operand A (128 rows, the
-// TMEM lanes) and all the tokens (up) or the expert's rows (down) as up to 64
-// columns, so no weight passes through registers. One pipeline serves both: a
-// step is two 128 x 128 weight tiles, an up task's gate and up tile of one
-// block or a down task's tiles of two blocks (of one, where the expert has more
-// than 16 rows).
+// TMEM lanes) and the expert's rows as columns, sixteen or up to 64 of them, so
+// no weight passes through registers; an up task gathers its tokens' codes. One
+// pipeline serves both: a step is two 128 x 128 weight tiles, an up task's gate
+// and up tile of one block or a down task's tiles of two blocks (of one, where
+// the expert has more than 16 rows).
 // Warps 0-3 and 8-11 take products out of TMEM and do the rest of a task, two
 // groups with a task each, so that one's end overlaps the other's products;
 // warp 4 loads weights and takes tasks, warp 5 issues MMAs, warp 6 loads
@@ -79,7 +80,11 @@ struct MoeWs {            // workspace layout
   float* hs;              // [P, blocks of f]
   float* up_part;         // [S1][2][P][f]
   float* dn_part;         // [S2][P][d]
+  int* inds;              // [T, k] choices, largest first (more than four tokens)
+  float* probs;           // [T, k]
   unsigned* next;         // next task; this and the following are zeroed by k_moe_route
+  unsigned* rt_next;      // next token to route
+  unsigned* routed;       // tokens routed
   unsigned* brought;      // [up tile] ranges brought
   unsigned* flag;         // [up tile] its block is quantised
   unsigned* dn_done;      // [tile of d] down tasks done
@@ -99,9 +104,11 @@ static long long layout_ws(uint8_t* w, int T, int d, int f, int E, int k, MoeWs*
   o->hs = reinterpret_cast<float*>(w), w += up16(4 * P * blocks128(f));
   o->up_part = reinterpret_cast<float*>(w), w += 8ll * o->cap1 * P * f;
   o->dn_part = reinterpret_cast<float*>(w), w += 4ll * o->cap2 * P * d;
-  o->next = reinterpret_cast<unsigned*>(w);
-  o->brought = o->next + 1, o->flag = o->brought + tiles, o->dn_done = o->flag + tiles;
-  o->counters = 1 + 2 * tiles + blocks128(d);
+  o->inds = reinterpret_cast<int*>(w), w += up16(4 * P);
+  o->probs = reinterpret_cast<float*>(w), w += up16(4 * P);
+  o->next = reinterpret_cast<unsigned*>(w), o->rt_next = o->next + 1, o->routed = o->next + 2;
+  o->brought = o->next + 3, o->flag = o->brought + tiles, o->dn_done = o->flag + tiles;
+  o->counters = 3 + 2 * tiles + blocks128(d);
   w += up16(4ll * o->counters);
   return w - w0;
 }
@@ -181,12 +188,13 @@ template <int NT> struct Moe {
   static constexpr int ACT = NT <= 32 ? 4096 : NT * 128;             // activation tiles of a step
   static constexpr int STAGE = 2 * FP8_W_TILE + ACT;
   static constexpr int STAGES = NT <= 32 ? 5 : 4;
-  static constexpr int BUFS = NT <= 32 ? 8 : 4;
+  static constexpr int BUFS = NT <= 32 ? 4 : 2;                      // of each group
   static constexpr int OFF_FAC = STAGES * STAGE;                     // [2][FAC][2][NT] scale products
   static constexpr int OFF_ROWS = OFF_FAC + 2 * MOE_FAC * 2 * NT * 4;   // [2][2][ROWS][128] gate and up sums
   static constexpr int OFF_PROB = OFF_ROWS + 2 * 2 * MOE_ROWS * 512; // [NT][32]
   static constexpr int OFF_IND = OFF_PROB + NT * 32 * 4;             // [NT][32] bytes
-  static constexpr int OFF_MASK = OFF_IND + NT * 32;                 // [256] tokens of an expert, 64 bits
+  static constexpr int OFF_TOK = OFF_IND + NT * 32;                  // [T * k] bytes, the rows' tokens
+  static constexpr int OFF_MASK = OFF_TOK + NT * 32;                 // [256] tokens of an expert, 64 bits
   static constexpr int OFF_START = OFF_MASK + 256 * 8;               // [256] its first row
   static constexpr int OFF_GROUP = OFF_START + 256 * 4;              // [256] experts that are routed to, ascending
   static constexpr int OFF_TASK = OFF_GROUP + 256;                   // [4] tasks
@@ -194,7 +202,7 @@ template <int NT> struct Moe {
   static constexpr int OFF_BAR = OFF_WORD + 64;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448 && SMEM > 232448 - 77824, "alone on its SM");
-  static_assert(STAGE % 1024 == 0 && BUFS * 2 * NT <= 512, "tile alignment, TMEM columns");
+  static_assert(STAGE % 1024 == 0 && 2 * BUFS * 2 * NT <= 512, "tile alignment, TMEM columns");
 };
 
 struct __align__(32) Task {
@@ -299,7 +307,7 @@ __device__ __forceinline__ bool wait_count(const unsigned* p, unsigned want) {
 }
 
 struct MoeMaps {
-  CUtensorMap gate, up, down, x, h, h16;
+  CUtensorMap gate, up, down, x, h;
 };
 
 template <int NT>
@@ -312,34 +320,36 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   float* s_fac = reinterpret_cast<float*>(smem + C::OFF_FAC);
   float* s_prob = reinterpret_cast<float*>(smem + C::OFF_PROB);
   uint8_t* s_ind = smem + C::OFF_IND;
+  uint8_t* s_tok = smem + C::OFF_TOK;
   unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::OFF_MASK);
   int* s_start = reinterpret_cast<int*>(smem + C::OFF_START);
   uint8_t* s_group = smem + C::OFF_GROUP;
-  volatile int* s_word = reinterpret_cast<volatile int*>(smem + C::OFF_WORD);   // last [2], groups, S1, S2
+  volatile int* s_word = reinterpret_cast<volatile int*>(smem + C::OFF_WORD);   // last [2][2], groups, S1, S2
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);        // [STAGES] both tiles landed
   uint64_t* empty = full + C::STAGES;                                     // [STAGES] read by the MMAs
-  uint64_t* d_full = empty + C::STAGES;                                   // [BUFS] a product complete
-  uint64_t* d_empty = d_full + C::BUFS;                                   // [BUFS] taken out
-  uint64_t* f_full = d_empty + C::BUFS;                                   // [2] a task's scales there
+  uint64_t* d_full = empty + C::STAGES;                                   // [2][BUFS] a group's product complete
+  uint64_t* d_empty = d_full + 2 * C::BUFS;                               // [2][BUFS] taken out
+  uint64_t* f_full = d_empty + 2 * C::BUFS;                                   // [2] a task's scales there
   uint64_t* f_empty = f_full + 2;                                         // [2] used
   uint64_t* t_full = f_empty + 2;                                         // [4] a task taken
   uint64_t* t_empty = t_full + 4;                                         // [4] done by all roles
   Task* s_task = reinterpret_cast<Task*>(smem + C::OFF_TASK);             // [4]
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(t_empty + 4);
+  uint64_t* g_bar = t_empty + 4;                                          // [2] a group's warps meet
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(g_bar + 2);
   int* const status = &g_moe_status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int P = a.T * a.k;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[i], 2), mbar_init(&empty[i], 1);
-    for (int i = 0; i < C::BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&f_full[i], 1), mbar_init(&f_empty[i], 4);
+    for (int i = 0; i < 2 * C::BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&f_full[i], 1), mbar_init(&f_empty[i], 4), mbar_init(&g_bar[i], 4);
     for (int i = 0; i < 4; ++i) mbar_init(&t_full[i], 1), mbar_init(&t_empty[i], 11);
     fence_barrier_init();
   }
   if (threadIdx.x < 256) s_mask[threadIdx.x] = 0;
   if (warp == 5) tmem_get(tmem_at, 512);
-  if (warp == 4 && lane < 6) tma_map_prefetch(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
+  if (warp == 4 && lane < 5) tma_map_prefetch(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
   tc_before();
   __syncthreads();
   tc_after();
@@ -391,8 +401,13 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (t + 1 < a.T) __syncthreads();
     }
   } else {
-    // a warp per token, the largest one after another
-    for (int t = warp; t < a.T; t += MOE_THREADS / 32) {
+    // tokens are shared out over the CTAs, a warp takes the largest logit one
+    // after another
+    while (warp == 0) {
+      int t = 0;
+      if (lane == 0) t = (int)atomicAdd(w.rt_next, 1u);
+      t = __shfl_sync(MS_FULL, t, 0);
+      if (t >= a.T) break;
       uint32_t key[8];
       float v[8];
       bool nan = false;
@@ -435,10 +450,19 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       const float p = lane < a.k ? expf(key_value(mine_key) - m) : 0.f;
       const float sel = warp_sum(p);
       if (lane < a.k) {
-        s_prob[t * 32 + lane] = p / (a.model == 1 || a.norm_topk ? sel : all);
-        s_ind[t * 32 + lane] = (uint8_t)mine;
-        atomicOr(&s_mask[mine], 1ull << t);
+        __stcg(w.probs + t * a.k + lane, p / (a.model == 1 || a.norm_topk ? sel : all));
+        __stcg(w.inds + t * a.k + lane, mine);
       }
+      __syncwarp();
+      if (lane == 0) red_release(w.routed);
+    }
+    if (threadIdx.x == 0) wait_count(w.routed, (unsigned)a.T);
+    __syncthreads();
+    for (int q = threadIdx.x; q < P; q += MOE_THREADS) {
+      const int t = q / a.k, j = q - t * a.k, e = __ldcg(w.inds + q) & 255;
+      s_prob[t * 32 + j] = __ldcg(w.probs + q);
+      s_ind[t * 32 + j] = (uint8_t)e;
+      atomicOr(&s_mask[e], 1ull << t);
     }
   }
   __syncthreads();
@@ -466,11 +490,16 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       }
     const int s1 = choose_split(G * blocks128(a.f), blocks128(a.d), gridDim.x, w.cap1, 2.f);
     const int s2 = choose_split(G * blocks128(a.d), blocks128(a.f), gridDim.x, w.cap2, 0.5f);
-    if (lane == 0) s_word[2] = G, s_word[3] = s1, s_word[4] = s2;
+    if (lane == 0) s_word[4] = G, s_word[5] = s1, s_word[6] = s2;
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < P; q += MOE_THREADS) {
+    const int t = q / a.k, e = s_ind[t * 32 + q - t * a.k];
+    s_tok[s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1))] = (uint8_t)t;
   }
   __syncthreads();
   Shape sh;
-  sh.G = s_word[2], sh.S1 = s_word[3], sh.S2 = s_word[4];
+  sh.G = s_word[4], sh.S1 = s_word[5], sh.S2 = s_word[6];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
   sh.n_up = sh.G * sh.FT * sh.S1, sh.n_dn = sh.G * sh.DT * sh.S2;
   sh.n_co = sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
@@ -481,25 +510,36 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   if (NT == 64 && warp >= 4 && warp < 8) regs_down<40>();
   if (warp == 4) {
     // ---- tasks and weight tiles
+    const uint64_t once = l2_evict_first();
     bool ok = true;
-    int i = 0;
-    for (int n = 0; ok; ++n) {
-      if (n >= 4) ok = mbar_wait_step(&t_empty[n & 3], ((n >> 2) - 1) & 1, status);
-      unsigned id = first_task;
-      if (n > 0 && lane == 0) id = ok ? atomicAdd(w.next, 1u) : 0xffffffffu;
-      id = __shfl_sync(MS_FULL, id, 0);
-      const Task t = sh.task(id);
+    int i = 0, n = 0;
+    auto take = [&](unsigned id) {           // the n-th task, published to the other warps
+      if (n >= 4 && !mbar_wait_step(&t_empty[n & 3], ((n >> 2) - 1) & 1, status)) ok = false;
+      const Task t = sh.task(ok ? id : 0xffffffffu);      // after a failure the other warps end
       if (lane == 0) {
         s_task[n & 3] = t;
         mbar_arrive1(&t_full[n & 3]);
       }
-      if (t.kind == 3) break;
+      ++n;
+      return t;
+    };
+    auto ticket = [&] {
+      unsigned id = 0;
+      if (lane == 0) id = atomicAdd(w.next, 1u);
+      return __shfl_sync(MS_FULL, id, 0);
+    };
+    Task t = take(__shfl_sync(MS_FULL, first_task, 0));
+    while (t.kind != 3) {
       if (t.kind == 2) {                     // one at a time, so that other CTAs take the next
-        ok = mbar_wait_step(&t_empty[n & 3], (n >> 2) & 1, status);
+        if (!mbar_wait_step(&t_empty[(n - 1) & 3], ((n - 1) >> 2) & 1, status)) ok = false;
+        t = take(ticket());
         continue;
       }
+      // the next task is known before this one's tiles are out: its scales and
+      // activations are fetched meanwhile
+      const Task next = take(ticket());
       const int e = s_group[t.g], per = t.kind == 0 ? 1 : down_per(t.g);
-      for (int b = t.b0; b < t.b1; b += per, ++i) {
+      for (int b = t.b0; b < t.b1 && ok; b += per, ++i) {
         const int s = i % C::STAGES;
         if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
           // copies in flight land before the CTA ends
@@ -512,20 +552,27 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
           const int tiles = t.kind == 0 ? 2 : min(per, t.b1 - b);
           mbar_expect_tx(&full[s], tiles * FP8_W_TILE);
           if (t.kind == 0) {
-            tma_tile_3d(at, &maps.gate, b * 128, t.tile * 128, e, &full[s]);
-            tma_tile_3d(at + FP8_W_TILE, &maps.up, b * 128, t.tile * 128, e, &full[s]);
+            tma_tile_3d_once(at, &maps.gate, b * 128, t.tile * 128, e, &full[s], once);
+            tma_tile_3d_once(at + FP8_W_TILE, &maps.up, b * 128, t.tile * 128, e, &full[s], once);
           } else {
             for (int h = 0; h < tiles; ++h)
-              tma_tile_3d(at + h * FP8_W_TILE, &maps.down, (b + h) * 128, t.tile * 128, e, &full[s]);
+              tma_tile_3d_once(at + h * FP8_W_TILE, &maps.down, (b + h) * 128, t.tile * 128, e, &full[s], once);
           }
         }
         __syncwarp();
       }
+      if (!ok) {
+        if (next.kind != 3) take(0);
+        break;
+      }
+      t = next;
     }
   } else if (warp == 5) {
-    // ---- MMAs
+    // ---- MMAs. Each group has buffers of its own and meets every phase of
+    // their barriers in turn: a wait for a parity does not tell a phase from
+    // the one two before it.
     bool ok = true;
-    int i = 0;
+    int i = 0, c = 0, j0 = 0, j1 = 0;        // steps; compute tasks; steps of each group
     for (int n = 0; ok; ++n) {
       if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
       const Task t = s_task[n & 3];
@@ -534,11 +581,13 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (t.kind == 3) break;
       if (t.kind == 2) continue;
       const int per = t.kind == 0 ? 1 : down_per(t.g);
-      const uint32_t idesc = t.kind == 1 && per == 2 ? idesc_e4m3(128, 16) : idesc_e4m3(128, NT);
+      const uint32_t idesc = idesc_e4m3(128, (__popcll(s_mask[s_group[t.g]]) + 15) & ~15);
+      const int grp = c++ & 1;
       for (int b = t.b0; b < t.b1; b += per, ++i) {
-        const int s = i % C::STAGES, u = i % C::BUFS;
+        const int j = grp ? j1++ : j0++;
+        const int s = i % C::STAGES, u = grp * C::BUFS + j % C::BUFS;
         if (!mbar_wait_step(&full[s], (i / C::STAGES) & 1, status) ||
-            (i >= C::BUFS && !mbar_wait_step(&d_empty[u], ((i / C::BUFS) - 1) & 1, status))) {
+            (j >= C::BUFS && !mbar_wait_step(&d_empty[u], ((j / C::BUFS) - 1) & 1, status))) {
           ok = false;
           break;
         }
@@ -569,11 +618,16 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
       if (t.kind == 3) break;
       if (t.kind == 2) continue;
-      const int start = s_start[s_group[t.g]], per = t.kind == 0 ? 1 : down_per(t.g);
+      const int e = s_group[t.g], start = s_start[e], rows = __popcll(s_mask[e]);
+      const int per = t.kind == 0 ? 1 : down_per(t.g);
+      int tok[4];                            // up: the tokens of rows 4 lane to 4 lane + 3, none beyond the last
       if (t.kind == 1) {
         for (int b = t.b0 + lane; b < t.b1; b += 32) wait_count(w.flag + t.g * sh.FT + b, 1);
         __syncwarp();
         fence_async_all();
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tok[q] = 4 * lane + q < rows ? s_tok[start + 4 * lane + q] : a.T;
       }
       for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int s = i % C::STAGES;
@@ -581,19 +635,17 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
           ok = false;
           break;
         }
-        if (elect_one()) {
-          uint8_t* at = smem + s * C::STAGE + 2 * FP8_W_TILE;
-          if (t.kind == 0) {
-            mbar_expect_tx(&full[s], NT * 128);
-            tma_tile_2d(at, &maps.x, b * 128, 0, &full[s]);
-          } else if (per == 1) {
-            mbar_expect_tx(&full[s], NT * 128);
-            tma_tile_2d(at, &maps.h, b * 128, start, &full[s]);
-          } else {
-            const int tiles = min(2, t.b1 - b);
-            mbar_expect_tx(&full[s], tiles * 2048);
-            for (int h = 0; h < tiles; ++h) tma_tile_2d(at + h * 2048, &maps.h16, (b + h) * 128, start, &full[s]);
-          }
+        uint8_t* at = smem + s * C::STAGE + 2 * FP8_W_TILE;
+        if (t.kind == 0) {
+          if (elect_one()) mbar_expect_tx(&full[s], (rows + 3) / 4 * 512);
+          __syncwarp();
+          if (4 * lane < rows) tma_gather4(at + lane * 512, &maps.x, b * 128, tok[0], tok[1], tok[2], tok[3], &full[s]);
+        } else if (elect_one()) {
+          const int tiles = min(per, t.b1 - b), boxes = (rows + 15) / 16;
+          mbar_expect_tx(&full[s], tiles * boxes * 2048);
+          for (int h = 0; h < tiles; ++h)
+            for (int q = 0; q < boxes; ++q)
+              tma_tile_2d(at + (h + q) * 2048, &maps.h, (b + h) * 128, start + 16 * q, &full[s]);
         }
         __syncwarp();
       }
@@ -619,8 +671,8 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         const float wg = __ldg(a.gate.s + at), wu = __ldg(a.up.s + at);
         if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
 #pragma unroll 8
-        for (int r = r0; r < a.T; r += 2) {
-          const float x = __ldcg(w.xs + r * sh.KB1 + b);
+        for (int r = r0; r < rows; r += 2) {
+          const float x = __ldcg(w.xs + s_tok[start + r] * sh.KB1 + b);
           if (wb < nb) fac[r] = x * wg, fac[NT + r] = x * wu;
         }
       } else {
@@ -641,9 +693,16 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   } else {
     // ---- products out of TMEM, and what follows them
     if (NT == 64) regs_up<232>();
-    const int grp = warp >> 3, tid = threadIdx.x & 127, bar = 1 + grp;
+    const int grp = warp >> 3, tid = threadIdx.x & 127;
     bool ok = true;
-    int i = 0, c = 0;
+    int i = 0, c = 0, met = 0, joins = 0;    // steps of this group; compute tasks
+    // the group's warps meet (a wait with a limit, unlike bar.sync)
+    auto meet = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&g_bar[grp]);
+      if (!mbar_wait_step(&g_bar[grp], met & 1, status)) ok = false;
+      ++met;
+    };
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float* s_rows = reinterpret_cast<float*>(smem + C::OFF_ROWS) + grp * (2 * MOE_ROWS * 128);
     float acc[2][NT];
@@ -659,7 +718,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         // y of four tokens, one per warp: rows in the order of the token's
         // choices, ranges in order
         if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2));
-        named_bar(bar, 128);
+        meet();
         const int f = t.tile * 128 + lane * 4, tok = t.s * COMBINE_T + warp;
         if (f < a.d && tok < a.T) {
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -707,14 +766,11 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       }
       const int per = t.kind == 0 ? 1 : down_per(t.g);
       if ((c & 1) != grp) {                  // the other group's
-        i += (t.b1 - t.b0 + per - 1) / per;
         ++c;
         continue;
       }
       const int e = s_group[t.g], start = s_start[e];
-      const unsigned long long mask = s_mask[e];
-      const int rows = __popcll(mask);
-      const int cols = t.kind == 0 ? a.T : rows;
+      const int rows = __popcll(s_mask[e]);
       const float* fac = s_fac + grp * (MOE_FAC * 2 * NT);
       ok = mbar_wait_step(&f_full[grp], (c >> 1) & 1, status);
 #pragma unroll
@@ -722,7 +778,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       auto take = [&](float* sum, uint32_t at, const float* f) {
 #pragma unroll
         for (int m = 0; m < NT; m += 16) {
-          if (m >= cols) break;
+          if (m >= rows) break;
           uint32_t v[16];
           tmem_load16(at + m, v);
           tmem_wait16(v);
@@ -738,7 +794,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
       };
       for (int b = t.b0; b < t.b1; b += per, ++i) {
-        const int u = i % C::BUFS;
+        const int u = grp * C::BUFS + i % C::BUFS;
         if (!ok || !mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, status)) {
           ok = false;
           break;
@@ -764,7 +820,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
 #pragma unroll
           for (int m = 0; m < NT; ++m)
             if (m < rows) __stcg(part + (long long)m * a.d, acc[0][m]);
-        named_bar(bar, 128);
+        meet();
         if (tid == 0) red_release(w.dn_done + t.tile);
         continue;
       }
@@ -773,21 +829,18 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         if (f < a.f) {
           float* pg = w.up_part + (t.s * 2ll * P + start) * a.f + f;
           float* pu = pg + (long long)P * a.f;
-          long long at = 0;
 #pragma unroll
           for (int m = 0; m < NT; ++m)
-            if (mask >> m & 1) {
-              __stcg(pg + at, acc[0][m]);
-              __stcg(pu + at, acc[1][m]);
-              at += a.f;
+            if (m < rows) {
+              __stcg(pg + (long long)m * a.f, acc[0][m]);
+              __stcg(pu + (long long)m * a.f, acc[1][m]);
             }
         }
-        named_bar(bar, 128);
-        if (tid == 0) s_word[grp] = add_acq_rel(w.brought + tile) == (unsigned)(sh.S1 - 1);
-        named_bar(bar, 128);
-        const bool last = s_word[grp];
-        named_bar(bar, 128);                 // all have read the word
-        if (!last) continue;
+        meet();
+        volatile int* last = s_word + 2 * grp + (joins++ & 1);
+        if (tid == 0) *last = add_acq_rel(w.brought + tile) == (unsigned)(sh.S1 - 1);
+        meet();
+        if (!*last) continue;
       }
       // a warp per row: four features a lane
       const int f4 = t.tile * 128 + lane * 4;
@@ -801,17 +854,16 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
       for (int r0 = 0; r0 < rows; r0 += MOE_ROWS) {
         if (sh.S1 == 1) {                    // this tile's sums are in the registers of their columns
-          int r = 0;
 #pragma unroll
-          for (int m = 0; m < NT; ++m)
-            if (mask >> m & 1) {
-              if (r >= r0 && r < r0 + MOE_ROWS) {
-                s_rows[(r - r0) * 128 + tid] = acc[0][m];
-                s_rows[(MOE_ROWS + r - r0) * 128 + tid] = acc[1][m];
+          for (int m = 0; m < NT; m += MOE_ROWS)
+            if (m == r0) {
+#pragma unroll
+              for (int q = 0; q < MOE_ROWS; ++q) {
+                s_rows[q * 128 + tid] = acc[0][m + q];
+                s_rows[(MOE_ROWS + q) * 128 + tid] = acc[1][m + q];
               }
-              ++r;
             }
-          named_bar(bar, 128);
+          meet();
         }
         for (int r = r0 + (warp & 3); r < min(rows, r0 + MOE_ROWS); r += 4) {
           float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
@@ -840,10 +892,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
                 e4m3x2(h0 * inv, h1 * inv) | e4m3x2(h2 * inv, h3 * inv) << 16;
           if (lane == 0) w.hs[(long long)(start + r) * sh.KB2 + t.tile] = s;
         }
-        if (sh.S1 == 1) named_bar(bar, 128); // the rows have been read
+        if (sh.S1 == 1) meet(); // the rows have been read
       }
       fence_async_all();                     // the codes are read by tensor copies
-      named_bar(bar, 128);
+      meet();
       if (tid == 0) red_release(w.flag + tile);
     }
   }
@@ -865,8 +917,7 @@ static cudaError_t launch_experts(const MoeFp8Args& a, const MoeWs& w, int sms, 
   if (encode_fp8_map(&m.gate, a.gate.q, a.d, a.f, a.d, 128, a.E, ew) ||
       encode_fp8_map(&m.up, a.up.q, a.d, a.f, a.d, 128, a.E, ew) ||
       encode_fp8_map(&m.down, a.down.q, a.f, a.d, a.f, 128, a.E, ew) ||
-      encode_fp8_map(&m.x, w.xq, a.d, a.T, a.d, NT, 0, 0) || encode_fp8_map(&m.h, w.hq, a.f, P, a.f, NT, 0, 0) ||
-      encode_fp8_map(&m.h16, w.hq, a.f, P, a.f, 16, 0, 0))
+      encode_fp8_map(&m.x, w.xq, a.d, a.T, a.d, 1, 0, 0) || encode_fp8_map(&m.h, w.hq, a.f, P, a.f, 16, 0, 0))
     return cudaErrorInvalidValue;
   auto kern = k_moe_experts<NT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Moe<NT>::SMEM);

@@ -316,7 +316,10 @@ def check_moe(y, x, router, rb, parts, k, model, norm=True, res=None):
     ("qwen3", 8, 512, 768, 60, 8), ("qwen3", 17, 128, 144, 128, 1), ("qwen3", 33, 768, 256, 8, 8),
     ("qwen3", 64, 256, 384, 12, 5), ("gptoss", 1, 2880, 720, 8, 4), ("gptoss", 2, 16, 16, 4, 4),
     ("gptoss", 5, 320, 320, 16, 4), ("gptoss", 64, 272, 400, 32, 4), ("gptoss", 40, 1024, 512, 3, 1),
-    ("qwen3", 64, 384, 128, 1, 1), ("qwen3", 2, 256, 256, 256, 32), ("gptoss", 64, 128, 128, 256, 32)])
+    ("qwen3", 64, 384, 128, 1, 1), ("qwen3", 2, 256, 256, 256, 32), ("gptoss", 64, 128, 128, 256, 32),
+    # many tasks on every SM, tiles cut into ranges by their length
+    ("qwen3", 16, 2048, 768, 128, 8), ("gptoss", 5, 2880, 1440, 32, 4), ("qwen3", 61, 1024, 512, 64, 8),
+    ("qwen3", 30, 2880, 2880, 4, 2)])
 def test_moe(model, T, d, f, E, k, lib, cuda):
     g = _gen(T + d + f + E)
     layer, router, rb, parts = make_moe(g, model, d, f, E, k)
