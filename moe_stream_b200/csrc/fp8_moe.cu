@@ -12,9 +12,9 @@
 //
 // Bound by memory: every routed expert's codes once. k_moe_route makes the
 // logits and x's codes; k_moe_experts streams the experts. Each of its CTAs
-// (one per SM) works out the routing of up to four tokens for itself, which is
-// less than a trip through memory; more tokens are shared out. Then it takes
-// tasks off one counter:
+// (one per SM) works out the routing of up to twelve tokens for itself, a warp
+// per token, which is less than a trip through memory; more tokens are shared
+// out. Then it takes tasks off one counter:
 //
 //   up       128 features of d_ff of one expert, gate and up rows, a range of
 //            the blocks of d (all of them where there are tiles enough; else
@@ -192,8 +192,8 @@ template <int NT> struct Moe {
   static constexpr int OFF_FAC = STAGES * STAGE;                     // [2][FAC][2][NT] scale products
   static constexpr int OFF_ROWS = OFF_FAC + 2 * MOE_FAC * 2 * NT * 4;   // [2][2][ROWS][128] gate and up sums
   static constexpr int OFF_PROB = OFF_ROWS + 2 * 2 * MOE_ROWS * 512; // [NT][32]
-  static constexpr int OFF_IND = OFF_PROB + NT * 32 * 4;             // [NT][32] bytes
-  static constexpr int OFF_TOK = OFF_IND + NT * 32;                  // [T * k] bytes, the rows' tokens
+  static constexpr int OFF_ROW = OFF_PROB + NT * 32 * 4;             // [NT][32] 16-bit: rows of the choices
+  static constexpr int OFF_TOK = OFF_ROW + NT * 64;                  // [T * k] bytes: tokens of the rows
   static constexpr int OFF_MASK = OFF_TOK + NT * 32;                 // [256] tokens of an expert, 64 bits
   static constexpr int OFF_START = OFF_MASK + 256 * 8;               // [256] its first row
   static constexpr int OFF_GROUP = OFF_START + 256 * 4;              // [256] experts that are routed to, ascending
@@ -284,14 +284,16 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-__device__ __forceinline__ float activate(int model, float g, float u) {
-  if (model == 1) {
-    g = g > 7.f ? 7.f : g;
-    u = u > 7.f ? 7.f : u < -7.f ? -7.f : u;
-    return g / (1.f + expf(-1.702f * g)) * (u + 1.f);
+// both models' activation: silu(g) u with alpha 1, beta 0, limit infinity;
+// gpt-oss alpha 1.702, beta 1, limit 7
+struct Act {
+  float alpha, beta, limit;
+  __device__ __forceinline__ float operator()(float g, float u) const {
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
+    return __fdividef(g, 1.f + expf(-alpha * g)) * (u + beta);
   }
-  return g / (1.f + expf(-g)) * u;
-}
+};
 __device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 // Waits until *p >= want, a second at most.
@@ -319,12 +321,12 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_fac = reinterpret_cast<float*>(smem + C::OFF_FAC);
   float* s_prob = reinterpret_cast<float*>(smem + C::OFF_PROB);
-  uint8_t* s_ind = smem + C::OFF_IND;
+  uint16_t* s_row = reinterpret_cast<uint16_t*>(smem + C::OFF_ROW);
   uint8_t* s_tok = smem + C::OFF_TOK;
   unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::OFF_MASK);
   int* s_start = reinterpret_cast<int*>(smem + C::OFF_START);
   uint8_t* s_group = smem + C::OFF_GROUP;
-  volatile int* s_word = reinterpret_cast<volatile int*>(smem + C::OFF_WORD);   // last [2][2], groups, S1, S2
+  volatile int* s_word = reinterpret_cast<volatile int*>(smem + C::OFF_WORD);   // last [2][2], S1, S2; [8] sums
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);        // [STAGES] both tiles landed
   uint64_t* empty = full + C::STAGES;                                     // [STAGES] read by the MMAs
   uint64_t* d_full = empty + C::STAGES;                                   // [2][BUFS] a group's product complete
@@ -359,54 +361,15 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   unsigned first_task = 0;
   if (warp == 4 && lane == 0) first_task = atomicAdd(w.next, 1u);    // back by the time it can be read
 
-  // ---- the routing
-  if (a.T <= 4) {
-    // few tokens: a thread per expert counts the logits above its own
-    uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + C::OFF_ROWS);
-    uint32_t* s_top = s_key + 256;
-    for (int t = 0; t < a.T; ++t) {
-      const int e = threadIdx.x;
-      const bool in = e < a.E;
-      const float v = in ? __ldcg(w.logits + t * a.E + e) + 0.f : 0.f;         // -0 is 0
-      const uint32_t key = in ? order_key(v) : 0u;
-      if (e < 256) s_key[e] = key;
-      const bool nan = __syncthreads_or(v != v);
-      if (in) {
-        int rank = 0;
-        for (int q = 0; q < a.E; q += 4) {
-          const uint4 o = *reinterpret_cast<const uint4*>(s_key + q);
-          rank += o.x > key || (o.x == key && q < e);
-          rank += o.y > key || (o.y == key && q + 1 < e);
-          rank += o.z > key || (o.z == key && q + 2 < e);
-          rank += o.w > key || (o.w == key && q + 3 < e);
-        }
-        if (rank < a.k) {
-          s_ind[t * 32 + rank] = (uint8_t)e;
-          s_top[rank] = key;
-          atomicOr(&s_mask[e], 1ull << t);
-        }
+  // ---- the routing: a warp per token takes the largest logit one after
+  // another. The code runs once, cold, so it is kept short.
+  const bool shared_out = a.T > MOE_THREADS / 32;
+  if (!shared_out || warp == 0)
+    for (int t = warp;; t = a.T) {
+      if (shared_out) {
+        if (lane == 0) t = (int)atomicAdd(w.rt_next, 1u);
+        t = __shfl_sync(MS_FULL, t, 0);
       }
-      __syncthreads();
-      if (warp == 0) {
-        const float m = nan ? __uint_as_float(0x7fc00000u) : key_value(s_top[0]);
-        const float p = lane < a.k ? expf(key_value(s_top[lane]) - m) : 0.f;
-        float sum = p;
-        if (a.model == 0 && !a.norm_topk) {
-          sum = 0.f;
-          for (int q = lane; q < a.E; q += 32) sum += expf(key_value(s_key[q]) - m);
-        }
-        sum = warp_sum(sum);
-        if (lane < a.k) s_prob[t * 32 + lane] = p / sum;
-      }
-      if (t + 1 < a.T) __syncthreads();
-    }
-  } else {
-    // tokens are shared out over the CTAs, a warp takes the largest logit one
-    // after another
-    while (warp == 0) {
-      int t = 0;
-      if (lane == 0) t = (int)atomicAdd(w.rt_next, 1u);
-      t = __shfl_sync(MS_FULL, t, 0);
       if (t >= a.T) break;
       uint32_t key[8];
       float v[8];
@@ -450,56 +413,64 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       const float p = lane < a.k ? expf(key_value(mine_key) - m) : 0.f;
       const float sel = warp_sum(p);
       if (lane < a.k) {
-        __stcg(w.probs + t * a.k + lane, p / (a.model == 1 || a.norm_topk ? sel : all));
-        __stcg(w.inds + t * a.k + lane, mine);
+        const float share = p / (a.model == 1 || a.norm_topk ? sel : all);
+        if (shared_out) {
+          __stcg(w.probs + t * a.k + lane, share);
+          __stcg(w.inds + t * a.k + lane, mine);
+        } else {
+          s_prob[t * 32 + lane] = share;
+          s_row[t * 32 + lane] = (uint16_t)mine;
+          atomicOr(&s_mask[mine], 1ull << t);
+        }
       }
       __syncwarp();
-      if (lane == 0) red_release(w.routed);
+      if (shared_out && lane == 0) red_release(w.routed);
+      if (!shared_out) break;
     }
+  if (shared_out) {
     if (threadIdx.x == 0) wait_count(w.routed, (unsigned)a.T);
     __syncthreads();
     for (int q = threadIdx.x; q < P; q += MOE_THREADS) {
-      const int t = q / a.k, j = q - t * a.k, e = __ldcg(w.inds + q) & 255;
-      s_prob[t * 32 + j] = __ldcg(w.probs + q);
-      s_ind[t * 32 + j] = (uint8_t)e;
+      const int t = q / a.k, at = t * 32 + q - t * a.k, e = __ldcg(w.inds + q) & 255;
+      s_prob[at] = __ldcg(w.probs + q);
+      s_row[at] = (uint16_t)e;
       atomicOr(&s_mask[e], 1ull << t);
     }
   }
   __syncthreads();
-  if (warp == 0) {                          // groups in expert order and their first rows, eight experts a lane
-    int n[8], sum = 0;                      // rows in the low half, groups in the high
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      n[i] = __popcll(s_mask[lane * 8 + i]);
-      sum += n[i] + (n[i] ? 1 << 16 : 0);
-    }
-    int at = sum;
+  // groups: the experts that have rows, ascending; their rows follow each other
+  const int mine_n = threadIdx.x < 256 ? __popcll(s_mask[threadIdx.x]) : 0;
+  const int G = __syncthreads_count(mine_n > 0);
+  if (warp < 8) {                           // rows in the low half, groups in the high; sums of the warps before
+    int at = mine_n + (mine_n ? 1 << 16 : 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(MS_FULL, at, o);
       if (lane >= o) at += u;
     }
-    const int G = __shfl_sync(MS_FULL, at, 31) >> 16;
-    at -= sum;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n[i]) {
-        s_group[at >> 16] = (uint8_t)(lane * 8 + i);
-        s_start[lane * 8 + i] = at & 0xffff;
-        at += n[i] + (1 << 16);
-      }
-    const int s1 = choose_split(G * blocks128(a.f), blocks128(a.d), gridDim.x, w.cap1, 2.f);
-    const int s2 = choose_split(G * blocks128(a.d), blocks128(a.f), gridDim.x, w.cap2, 0.5f);
-    if (lane == 0) s_word[4] = G, s_word[5] = s1, s_word[6] = s2;
+    if (lane == 31) s_word[8 + warp] = at;
+    named_bar(1, 256);
+    for (int q = 0; q < warp; ++q) at += s_word[8 + q];
+    if (mine_n) {
+      s_group[(at >> 16) - 1] = (uint8_t)threadIdx.x;
+      s_start[threadIdx.x] = (at & 0xffff) - mine_n;
+    }
+  } else if (warp < 10) {
+    const int nf = blocks128(a.f), nd = blocks128(a.d);
+    const int split = warp == 8 ? choose_split(G * nf, nd, gridDim.x, w.cap1, 2.f)
+                                : choose_split(G * nd, nf, gridDim.x, w.cap2, 0.5f);
+    if (lane == 0) s_word[warp - 4] = split;
   }
   __syncthreads();
-  for (int q = threadIdx.x; q < P; q += MOE_THREADS) {
-    const int t = q / a.k, e = s_ind[t * 32 + q - t * a.k];
-    s_tok[s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1))] = (uint8_t)t;
+  for (int q = threadIdx.x; q < P; q += MOE_THREADS) {     // a choice's row, a row's token
+    const int t = q / a.k, at = t * 32 + q - t * a.k, e = s_row[at];
+    const int row = s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1));
+    s_row[at] = (uint16_t)row;
+    s_tok[row] = (uint8_t)t;
   }
   __syncthreads();
   Shape sh;
-  sh.G = s_word[4], sh.S1 = s_word[5], sh.S2 = s_word[6];
+  sh.G = G, sh.S1 = s_word[4], sh.S2 = s_word[5];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
   sh.n_up = sh.G * sh.FT * sh.S1, sh.n_dn = sh.G * sh.DT * sh.S2;
   sh.n_co = sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
@@ -722,34 +693,28 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         const int f = t.tile * 128 + lane * 4, tok = t.s * COMBINE_T + warp;
         if (f < a.d && tok < a.T) {
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          const unsigned long long below = (1ull << tok) - 1;
+          const float* const p0 = w.dn_part + f;
           for (int j0 = 0; j0 < a.k; j0 += 8) {
             float4 o[8];
-            const float* part[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < sh.S2; ++s) {
+              const int r0 = s * P;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int row = r0 + s_row[tok * 32 + min(j0 + j, a.k - 1)];
+                const float4 u = __ldcg(reinterpret_cast<const float4*>(p0 + (long long)row * a.d));
+                o[j].x += u.x, o[j].y += u.y, o[j].z += u.z, o[j].w += u.w;
+              }
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int e = s_ind[tok * 32 + min(j0 + j, a.k - 1)];
-              part[j] = w.dn_part + (long long)(s_start[e] + __popcll(s_mask[e] & below)) * a.d + f;
-              o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            for (int s = 0; s < sh.S2; ++s) {
-              float4 u[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) u[j] = __ldcg(reinterpret_cast<const float4*>(part[j] + s * (long long)P * a.d));
-#pragma unroll
-              for (int j = 0; j < 8; ++j) o[j].x += u[j].x, o[j].y += u[j].y, o[j].z += u[j].z, o[j].w += u[j].w;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
+              const float p = j0 + j < a.k ? s_prob[tok * 32 + j0 + j] : 0.f;
               if (j0 + j < a.k) {
-                const float p = s_prob[tok * 32 + j0 + j];
-                if (a.down.bias) {
-                  const float* b = a.down.bias + (long long)s_ind[tok * 32 + j0 + j] * a.d + f;
-                  o[j].x += __ldg(b), o[j].y += __ldg(b + 1), o[j].z += __ldg(b + 2), o[j].w += __ldg(b + 3);
-                }
                 y.x = fmaf(p, o[j].x, y.x), y.y = fmaf(p, o[j].y, y.y);
                 y.z = fmaf(p, o[j].z, y.z), y.w = fmaf(p, o[j].w, y.w);
               }
+            }
           }
           const long long at = (long long)tok * a.d + f;
           if (a.res) {
@@ -816,10 +781,11 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       const int f = t.tile * 128 + tid;
       if (t.kind == 1) {
         float* part = w.dn_part + (t.s * (long long)P + start) * a.d + f;
+        const float bias = t.s == 0 && a.down.bias && f < a.d ? __ldg(a.down.bias + (long long)e * a.d + f) : 0.f;
         if (f < a.d)
 #pragma unroll
           for (int m = 0; m < NT; ++m)
-            if (m < rows) __stcg(part + (long long)m * a.d, acc[0][m]);
+            if (m < rows) __stcg(part + (long long)m * a.d, acc[0][m] + bias);
         meet();
         if (tid == 0) red_release(w.dn_done + t.tile);
         continue;
@@ -843,6 +809,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         if (!*last) continue;
       }
       // a warp per row: four features a lane
+      const Act act = a.model == 1 ? Act{1.702f, 1.f, 7.f} : Act{1.f, 0.f, __uint_as_float(0x7f800000u)};
       const int f4 = t.tile * 128 + lane * 4;
       const bool in = f4 < a.f;
       float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
@@ -880,10 +847,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
               u.x += y.x, u.y += y.y, u.z += y.z, u.w += y.w;
             }
           }
-          const float h0 = in ? activate(a.model, g.x + bg[0], u.x + bu[0]) : 0.f;
-          const float h1 = in ? activate(a.model, g.y + bg[1], u.y + bu[1]) : 0.f;
-          const float h2 = in ? activate(a.model, g.z + bg[2], u.z + bu[2]) : 0.f;
-          const float h3 = in ? activate(a.model, g.w + bg[3], u.w + bu[3]) : 0.f;
+          const float h0 = in ? act(g.x + bg[0], u.x + bu[0]) : 0.f;
+          const float h1 = in ? act(g.y + bg[1], u.y + bu[1]) : 0.f;
+          const float h2 = in ? act(g.z + bg[2], u.z + bu[2]) : 0.f;
+          const float h3 = in ? act(g.w + bg[3], u.w + bu[3]) : 0.f;
           float inv;
           const float s = group_scale(
               warp_max(max_nan(max_nan(fabsf(h0), fabsf(h1)), max_nan(fabsf(h2), fabsf(h3)))), &inv);
