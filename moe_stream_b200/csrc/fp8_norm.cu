@@ -10,18 +10,19 @@
 // border is the same whatever the launch shape. Everything after it is one
 // 32-bit rounding per product.
 //
-// Bound by memory: x, res, h and the codes once each. A row stays in
-// registers between the sum and the codes. Eight consecutive features per
-// thread: 16 lanes make a group, its maximum is four shuffles.
+// Bound by memory: x, res, h and the codes once each. A CTA owns a row at a
+// time and keeps it in registers between the sum and the codes, the weight
+// too, from row to row. Eight consecutive features per thread and chunk: 16
+// lanes make a group, its maximum is four shuffles.
+#include <algorithm>
+
 #include <cuda_fp16.h>
 
 #include "fp8.cuh"
 
 namespace ms {
 
-template <int DT> struct Elem;
-template <> struct Elem<DT_BF16> { using T = uint16_t; };
-template <> struct Elem<DT_F16> { using T = uint16_t; };
+template <int DT> struct Elem { using T = uint16_t; };
 template <> struct Elem<DT_F32> { using T = float; };
 
 template <int DT>
@@ -38,90 +39,196 @@ __device__ __forceinline__ float elem_round(float v) {
   else return bfr(v);
 }
 template <int DT>
-__device__ __forceinline__ void elem_store(typename Elem<DT>::T* p, float v) {
-  if constexpr (DT == DT_F32) *p = v;
-  else if constexpr (DT == DT_F16) *p = __half_as_ushort(__float2half_rn(v));
-  else *p = f2bf(v);
+__device__ __forceinline__ uint16_t elem_bits(float v) {
+  if constexpr (DT == DT_F16) return __half_as_ushort(__float2half_rn(v));
+  else return f2bf(v);
 }
 
-// Row values of chunk c (8 features from 8c); features past d read as 0.
-template <int DT>
+// Features 8c to 8c + 7 of a row; those past d read as 0. VEC: whole chunks,
+// rows on 16-byte boundaries.
+template <int DT, bool VEC>
 __device__ __forceinline__ void load8(const typename Elem<DT>::T* row, int c, int d, float* v) {
+  if constexpr (VEC && DT == DT_F32) {
+    const float4 a = reinterpret_cast<const float4*>(row)[2 * c], b = reinterpret_cast<const float4*>(row)[2 * c + 1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else if constexpr (VEC) {
+    const uint4 a = reinterpret_cast<const uint4*>(row)[c];
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 8 * c + i < d ? elem_load<DT>(row + 8 * c + i) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == DT_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 8 * c + i < d ? elem_load<DT>(row + 8 * c + i) : 0.f;
+  }
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(typename Elem<DT>::T* row, int c, int d, const float* v) {
+  if constexpr (VEC && DT == DT_F32) {
+    reinterpret_cast<float4*>(row)[2 * c] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(row)[2 * c + 1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else if constexpr (VEC) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = elem_bits<DT>(v[2 * i]) | (uint32_t)elem_bits<DT>(v[2 * i + 1]) << 16;
+    reinterpret_cast<uint4*>(row)[c] = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (8 * c + i < d) {
+        if constexpr (DT == DT_F32) row[8 * c + i] = v[i];
+        else row[8 * c + i] = elem_bits<DT>(v[i]);
+      }
+  }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(256) k_norm_fp8(NormArgs a) {
+// NC chunks per thread; chunk i of a thread is threadIdx.x + i * blockDim.x,
+// so the 16 lanes of a group are neighbours.
+template <int DT, int NC, bool NORM, bool VEC>
+__global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
   using E = typename Elem<DT>::T;
-  __shared__ double red[8];
+  __shared__ double red[2][16];
   const int d = a.d, chunks = (d + 7) / 8, groups = (d + FP8_BLOCK - 1) / FP8_BLOCK;
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  float w[NORM ? NC : 1][8];
+  if constexpr (NORM)
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[i][j] = 0.f;
+      if (c < chunks) load8<DT, VEC>(static_cast<const E*>(a.w), c, d, w[i]);
+    }
+  int turn = 0;
+  for (int t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
     const E* x = static_cast<const E*>(a.x) + t * a.x_stride;
-    const E* r = a.res ? static_cast<const E*>(a.res) + t * a.res_stride : nullptr;
-    auto row8 = [&](int c, float* v) {
-      load8<DT>(x, c, d, v);
-      if (r) {
-        float u[8];
-        load8<DT>(r, c, d, u);
+    float v[NC][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = elem_round<DT>(__fadd_rn(v[i], u[i]));
-      }
-    };
+    for (int i = 0; i < NC; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      if (c < chunks) load8<DT, VEC>(x, c, d, v[i]);
+    }
     float f = 1.f;
-    if (a.w) {
-      double ss = 0.0;
-      for (int c = threadIdx.x; c < chunks; c += 256) {
-        float v[8];
-        row8(c, v);
+    if constexpr (NORM) {
+      if (a.res) {
+        const E* r = static_cast<const E*>(a.res) + t * a.res_stride;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
+        for (int i = 0; i < NC; ++i) {
+          const int c = threadIdx.x + i * blockDim.x;
+          if (c < chunks) {
+            float u[8];
+            load8<DT, VEC>(r, c, d, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = elem_round<DT>(__fadd_rn(v[i][j], u[j]));
+            store8<DT, VEC>(static_cast<E*>(a.h) + t * a.h_stride, c, d, v[i]);
+          }
+        }
       }
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fma((double)v[i][j], (double)v[i][j], ss);
 #pragma unroll
       for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(MS_FULL, ss, o);
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-      __syncthreads();
-      ss = 0.0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += red[i];
+      if (warps > 1) {                      // two sets of sums: one barrier a row
+        if (lane == 0) red[turn][warp] = ss;
+        __syncthreads();
+        ss = 0.0;
+        for (int i = 0; i < warps; ++i) ss += red[turn][i];
+      }
       f = (float)(1.0 / sqrt(ss / (double)d + a.eps));
     }
-    // every lane of a group's 16 takes part in its maximum
-    for (int c = threadIdx.x; c < groups * 16; c += 256) {
-      float v[8];
-      row8(c, v);
-      if (a.h)
-        for (int i = 0; i < 8 && 8 * c + i < d; ++i)
-          elem_store<DT>(static_cast<E*>(a.h) + t * a.h_stride + 8 * c + i, v[i]);
+    uint8_t* q = a.q + t * a.q_stride;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
       float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (a.w && 8 * c + i < d)
-          v[i] = __fmul_rn(__fmul_rn(v[i], f), elem_load<DT>(static_cast<const E*>(a.w) + 8 * c + i));
-        m = max_nan(m, fabsf(v[i]));
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (NORM) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], f), w[i][j]);
+        if (VEC || 8 * c + j < d) m = max_nan(m, fabsf(v[i][j]));      // past d: 0 times an infinite factor
       }
-      if (a.y)
-        for (int i = 0; i < 8 && 8 * c + i < d; ++i)
-          elem_store<DT>(static_cast<E*>(a.y) + t * a.y_stride + 8 * c + i, v[i]);
-      const unsigned lanes = 0xffffu << (threadIdx.x & 16);
+      if (NORM && a.y && c < chunks) store8<DT, VEC>(static_cast<E*>(a.y) + t * a.y_stride, c, d, v[i]);
+      if (VEC && c >= chunks) m = 0.f;
 #pragma unroll
-      for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(lanes, m, o));
+      for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(MS_FULL, m, o));
       float inv;
       const float s = group_scale(m, &inv);
-      if ((threadIdx.x & 15) == 0) a.s[(long long)t * groups + c / 16] = s;
-      for (int i = 0; i < 8 && 8 * c + i < d; ++i)
-        a.q[t * a.q_stride + 8 * c + i] = (uint8_t)e4m3x2(v[i] * inv, 0.f);
+      if ((threadIdx.x & 15) == 0 && c / 16 < groups) a.s[(long long)t * groups + c / 16] = s;
+      if (c < chunks) {
+        if constexpr (VEC) {
+          uint32_t b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = e4m3x2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv);
+          reinterpret_cast<uint2*>(q)[c] = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (8 * c + j < d) q[8 * c + j] = (uint8_t)e4m3x2(v[i][j] * inv, 0.f);
+        }
+      }
     }
   }
 }
 
+template <int DT, int NC, bool NORM, bool VEC>
+static cudaError_t launch_nc(const NormArgs& a, int threads, int grid, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_norm_fp8<DT, NC, NORM, VEC>, a);
+}
+
+template <int DT, bool NORM, bool VEC>
+static cudaError_t launch_vec(const NormArgs& a, int sms, cudaStream_t s) {
+  const int chunks = (a.d + 7) / 8, whole = (chunks + 31) / 32 * 32;
+  // Rows enough to fill the GPU: three chunks a thread, so that a row's
+  // barriers and its ragged end cost little; few rows: as many threads as
+  // there are chunks.
+  const bool many = a.T >= sms * 4;
+  int nc = many ? 3 : 1;
+  while ((whole + nc - 1) / nc > 512) ++nc;
+  const int threads = std::max(32, ((chunks + nc - 1) / nc + 31) / 32 * 32);
+  const int per_sm = std::max(1, 2048 / threads);
+  const int grid = (int)std::min<long long>(a.T, (long long)sms * per_sm);
+  if (nc == 1) return launch_nc<DT, 1, NORM, VEC>(a, threads, grid, s);
+  if (nc == 2) return launch_nc<DT, 2, NORM, VEC>(a, threads, grid, s);
+  if (nc == 3) return launch_nc<DT, 3, NORM, VEC>(a, threads, grid, s);
+  return launch_nc<DT, 4, NORM, VEC>(a, threads, grid, s);      // 16384 features / 8 / 512
+}
+
+template <int DT>
+static cudaError_t launch_dt(const NormArgs& a, int sms, cudaStream_t s) {
+  constexpr int PER = DT == DT_F32 ? 4 : 8;      // elements of 16 bytes
+  auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+  const bool vec = a.d % 8 == 0 && !off(a.x) && !off(a.res) && !off(a.w) && !off(a.h) && !off(a.y) && !off(a.q) &&
+                   a.x_stride % PER == 0 && (!a.res || a.res_stride % PER == 0) && (!a.h || a.h_stride % PER == 0) &&
+                   (!a.y || a.y_stride % PER == 0) && a.q_stride % 8 == 0;
+  if (a.w) return vec ? launch_vec<DT, true, true>(a, sms, s) : launch_vec<DT, true, false>(a, sms, s);
+  return vec ? launch_vec<DT, false, true>(a, sms, s) : launch_vec<DT, false, false>(a, sms, s);
+}
+
 cudaError_t launch_norm_fp8(const NormArgs& a, int dtype, int sms, cudaStream_t s) {
-  const int grid = a.T < sms * 8 ? a.T : sms * 8;
-  if (dtype == DT_BF16) k_norm_fp8<DT_BF16><<<grid, 256, 0, s>>>(a);
-  else if (dtype == DT_F16) k_norm_fp8<DT_F16><<<grid, 256, 0, s>>>(a);
-  else k_norm_fp8<DT_F32><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError();
+  if (dtype == DT_BF16) return launch_dt<DT_BF16>(a, sms, s);
+  if (dtype == DT_F16) return launch_dt<DT_F16>(a, sms, s);
+  return launch_dt<DT_F32>(a, sms, s);
 }
 
 }  // namespace ms
