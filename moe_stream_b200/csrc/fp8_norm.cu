@@ -31,61 +31,88 @@ __device__ __forceinline__ float elem_load(const typename Elem<DT>::T* p) {
   else if constexpr (DT == DT_F16) return __half2float(__ushort_as_half(*p));
   else return bf2f(*p);
 }
-// v rounded to the type, as a float
-template <int DT>
-__device__ __forceinline__ float elem_round(float v) {
-  if constexpr (DT == DT_F32) return v;
-  else if constexpr (DT == DT_F16) return __half2float(__float2half_rn(v));
-  else return bfr(v);
-}
 template <int DT>
 __device__ __forceinline__ uint16_t elem_bits(float v) {
   if constexpr (DT == DT_F16) return __half_as_ushort(__float2half_rn(v));
   else return f2bf(v);
 }
 
-// Features 8c to 8c + 7 of a row; those past d read as 0. VEC: whole chunks,
-// rows on 16-byte boundaries.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* row, int c, int d, float* v) {
-  if constexpr (VEC && DT == DT_F32) {
-    const float4 a = reinterpret_cast<const float4*>(row)[2 * c], b = reinterpret_cast<const float4*>(row)[2 * c + 1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else if constexpr (VEC) {
-    const uint4 a = reinterpret_cast<const uint4*>(row)[c];
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+// Eight features as they lie in memory: half the registers of their values
+// for the 16-bit types.
+template <int DT> struct Raw { uint32_t u[4]; };
+template <> struct Raw<DT_F32> { uint32_t u[8]; };
+
+template <int DT>
+__device__ __forceinline__ void unpack(const Raw<DT>& r, float* v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == DT_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      }
+  for (int i = 0; i < (DT == DT_F32 ? 8 : 4); ++i) {
+    if constexpr (DT == DT_F32) {
+      v[i] = __uint_as_float(r.u[i]);
+    } else if constexpr (DT == DT_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.u[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = __uint_as_float(r.u[i] << 16), v[2 * i + 1] = __uint_as_float(r.u[i] & 0xffff0000u);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 8 * c + i < d ? elem_load<DT>(row + 8 * c + i) : 0.f;
   }
 }
-template <int DT, bool VEC>
-__device__ __forceinline__ void store8(typename Elem<DT>::T* row, int c, int d, const float* v) {
-  if constexpr (VEC && DT == DT_F32) {
-    reinterpret_cast<float4*>(row)[2 * c] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(row)[2 * c + 1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else if constexpr (VEC) {
-    uint32_t u[4];
+// rounded to the type
+template <int DT>
+__device__ __forceinline__ Raw<DT> pack(const float* v) {
+  Raw<DT> r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = elem_bits<DT>(v[2 * i]) | (uint32_t)elem_bits<DT>(v[2 * i + 1]) << 16;
-    reinterpret_cast<uint4*>(row)[c] = make_uint4(u[0], u[1], u[2], u[3]);
+  for (int i = 0; i < (DT == DT_F32 ? 8 : 4); ++i) {
+    if constexpr (DT == DT_F32) r.u[i] = __float_as_uint(v[i]);
+    else r.u[i] = elem_bits<DT>(v[2 * i]) | (uint32_t)elem_bits<DT>(v[2 * i + 1]) << 16;
+  }
+  return r;
+}
+// Features 8c to 8c + 7 of a row; those past d are 0. VEC: whole chunks, rows
+// on 16-byte boundaries.
+template <int DT, bool VEC>
+__device__ __forceinline__ Raw<DT> load8(const typename Elem<DT>::T* row, int c, int d) {
+  Raw<DT> r;
+  if constexpr (VEC) {
+    const uint4* p = reinterpret_cast<const uint4*>(row) + (DT == DT_F32 ? 2 : 1) * c;
+#pragma unroll
+    for (int i = 0; i < (DT == DT_F32 ? 2 : 1); ++i) {
+      const uint4 a = p[i];
+      r.u[4 * i] = a.x, r.u[4 * i + 1] = a.y, r.u[4 * i + 2] = a.z, r.u[4 * i + 3] = a.w;
+    }
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 8 * c + i < d ? elem_load<DT>(row + 8 * c + i) : 0.f;
+    r = pack<DT>(v);
+  }
+  return r;
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(typename Elem<DT>::T* row, int c, int d, const Raw<DT>& r) {
+  if constexpr (VEC) {
+    uint4* p = reinterpret_cast<uint4*>(row) + (DT == DT_F32 ? 2 : 1) * c;
+#pragma unroll
+    for (int i = 0; i < (DT == DT_F32 ? 2 : 1); ++i)
+      p[i] = make_uint4(r.u[4 * i], r.u[4 * i + 1], r.u[4 * i + 2], r.u[4 * i + 3]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (8 * c + i < d) {
-        if constexpr (DT == DT_F32) row[8 * c + i] = v[i];
-        else row[8 * c + i] = elem_bits<DT>(v[i]);
+        if constexpr (DT == DT_F32) row[8 * c + i] = __uint_as_float(r.u[i]);
+        else row[8 * c + i] = (uint16_t)(r.u[i / 2] >> (16 * (i & 1)));
       }
   }
+}
+
+// 1 / sqrt(m), rounded once to 32 bits: two Newton steps in 64 from the 32-bit
+// estimate (relative error below 1e-13, far below half a step of the result),
+// a few instructions where the 64-bit root and quotient take many.
+__device__ __forceinline__ float rms_factor(double m) {
+  if (!(m > 1e-37 && m < 1e37)) return (float)(1.0 / sqrt(m));
+  double y = (double)rsqrtf((float)m);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-m * y, y, 1.0), y);
+  return (float)y;
 }
 
 // NC chunks per thread; chunk i of a thread is threadIdx.x + i * blockDim.x,
@@ -98,47 +125,56 @@ __global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  float w[NORM ? NC : 1][8];
+  Raw<DT> w[NORM ? NC : 1];
   if constexpr (NORM)
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[i][j] = 0.f;
-      if (c < chunks) load8<DT, VEC>(static_cast<const E*>(a.w), c, d, w[i]);
+      w[i] = {};
+      if (c < chunks) w[i] = load8<DT, VEC>(static_cast<const E*>(a.w), c, d);
     }
   int turn = 0;
   for (int t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
     const E* x = static_cast<const E*>(a.x) + t * a.x_stride;
-    float v[NC][8];
+    Raw<DT> h[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      if (c < chunks) load8<DT, VEC>(x, c, d, v[i]);
+      h[i] = {};
+      if (c < chunks) h[i] = load8<DT, VEC>(x, c, d);
     }
     float f = 1.f;
     if constexpr (NORM) {
       if (a.res) {
         const E* r = static_cast<const E*>(a.res) + t * a.res_stride;
+        Raw<DT> u[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int c = threadIdx.x + i * blockDim.x;
+          if (c < chunks) u[i] = load8<DT, VEC>(r, c, d);
+        }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           const int c = threadIdx.x + i * blockDim.x;
           if (c < chunks) {
-            float u[8];
-            load8<DT, VEC>(r, c, d, u);
+            float p[8], q[8];
+            unpack<DT>(h[i], p);
+            unpack<DT>(u[i], q);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = elem_round<DT>(__fadd_rn(v[i][j], u[j]));
-            store8<DT, VEC>(static_cast<E*>(a.h) + t * a.h_stride, c, d, v[i]);
+            for (int j = 0; j < 8; ++j) p[j] = __fadd_rn(p[j], q[j]);
+            h[i] = pack<DT>(p);
+            store8<DT, VEC>(static_cast<E*>(a.h) + t * a.h_stride, c, d, h[i]);
           }
         }
       }
       double ss = 0.0;
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        float v[8];
+        unpack<DT>(h[i], v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fma((double)v[i][j], (double)v[i][j], ss);
+        for (int j = 0; j < 8; ++j) ss = fma((double)v[j], (double)v[j], ss);
+      }
 #pragma unroll
       for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(MS_FULL, ss, o);
       if (warps > 1) {                      // two sets of sums: one barrier a row
@@ -147,19 +183,24 @@ __global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
         ss = 0.0;
         for (int i = 0; i < warps; ++i) ss += red[turn][i];
       }
-      f = (float)(1.0 / sqrt(ss / (double)d + a.eps));
+      f = rms_factor(ss / (double)d + a.eps);
     }
     uint8_t* q = a.q + t * a.q_stride;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-      float m = 0.f;
+      float v[8], m = 0.f;
+      unpack<DT>(h[i], v);
+      if constexpr (NORM) {
+        float g[8];
+        unpack<DT>(w[i], g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (NORM) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], f), w[i][j]);
-        if (VEC || 8 * c + j < d) m = max_nan(m, fabsf(v[i][j]));      // past d: 0 times an infinite factor
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], f), g[j]);
       }
-      if (NORM && a.y && c < chunks) store8<DT, VEC>(static_cast<E*>(a.y) + t * a.y_stride, c, d, v[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (VEC || 8 * c + j < d) m = max_nan(m, fabsf(v[j]));      // past d: 0 times an infinite factor
+      if (NORM && a.y && c < chunks) store8<DT, VEC>(static_cast<E*>(a.y) + t * a.y_stride, c, d, pack<DT>(v));
       if (VEC && c >= chunks) m = 0.f;
 #pragma unroll
       for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(MS_FULL, m, o));
@@ -170,12 +211,12 @@ __global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
         if constexpr (VEC) {
           uint32_t b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = e4m3x2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv);
+          for (int j = 0; j < 4; ++j) b[j] = e4m3x2(v[2 * j] * inv, v[2 * j + 1] * inv);
           reinterpret_cast<uint2*>(q)[c] = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (8 * c + j < d) q[8 * c + j] = (uint8_t)e4m3x2(v[i][j] * inv, 0.f);
+            if (8 * c + j < d) q[8 * c + j] = (uint8_t)e4m3x2(v[j] * inv, 0.f);
         }
       }
     }
