@@ -27,11 +27,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // Both are NaN when a is an infinity or a NaN, which makes every code of the
 // group NaN.
 __device__ __forceinline__ float group_scale(float a, float* inv) {
-  const uint32_t b = __float_as_uint(a < 7.88860905e-31f ? 7.88860905e-31f : a);   // 2^-100
-  if ((b >> 23) >= 255u) return *inv = __uint_as_float(0x7fc00000u);
-  const uint32_t e = (b >> 23) - 8u + ((b & 0x7fffffu) > 0x600000u ? 1u : 0u);
-  *inv = __uint_as_float((254u - e) << 23);
-  return __uint_as_float(e << 23);
+  const uint32_t b = __float_as_uint(max_nan(a, 7.88860905e-31f));   // 2^-100
+  // the carry out of the fraction is the step from 1.75 to the next exponent
+  const uint32_t e = (b + 0x1fffffu) & 0xff800000u;
+  const bool bad = b >= 0x7f800000u;
+  *inv = __uint_as_float(bad ? 0x7fc00000u : (262u << 23) - e);
+  return __uint_as_float(bad ? 0x7fc00000u : e - (8u << 23));
 }
 
 // two floats -> two e4m3 codes (lo in the low byte), nearest even; NaN -> 0x7f

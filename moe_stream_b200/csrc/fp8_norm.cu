@@ -31,12 +31,6 @@ __device__ __forceinline__ float elem_load(const typename Elem<DT>::T* p) {
   else if constexpr (DT == DT_F16) return __half2float(__ushort_as_half(*p));
   else return bf2f(*p);
 }
-template <int DT>
-__device__ __forceinline__ uint16_t elem_bits(float v) {
-  if constexpr (DT == DT_F16) return __half_as_ushort(__float2half_rn(v));
-  else return f2bf(v);
-}
-
 // Eight features as they lie in memory: half the registers of their values
 // for the 16-bit types.
 template <int DT> struct Raw { uint32_t u[4]; };
@@ -62,8 +56,15 @@ __device__ __forceinline__ Raw<DT> pack(const float* v) {
   Raw<DT> r;
 #pragma unroll
   for (int i = 0; i < (DT == DT_F32 ? 8 : 4); ++i) {
-    if constexpr (DT == DT_F32) r.u[i] = __float_as_uint(v[i]);
-    else r.u[i] = elem_bits<DT>(v[2 * i]) | (uint32_t)elem_bits<DT>(v[2 * i + 1]) << 16;
+    if constexpr (DT == DT_F32) {
+      r.u[i] = __float_as_uint(v[i]);
+    } else if constexpr (DT == DT_F16) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      r.u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      r.u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
   }
   return r;
 }
@@ -104,6 +105,32 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* row, int c, int d, 
   }
 }
 
+// The sum of eight squares, in 64 bits.
+__device__ __forceinline__ double squares(const float* v) {
+  double ss[2] = {0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double x = (double)v[i];
+    ss[i & 1] = fma(x, x, ss[i & 1]);
+  }
+  return ss[0] + ss[1];
+}
+// largest of |v|, NaN where one is
+__device__ __forceinline__ float max8_nan(const float* v) {
+  float m = fabsf(v[0]);
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[1])), "f"(fabsf(v[2])));
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[3])), "f"(fabsf(v[4])));
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[5])), "f"(fabsf(v[6])));
+  return max_nan(m, fabsf(v[7]));
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+  uint64_t p, q;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(x), "f"(y));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(p) : "l"(q));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+
 // 1 / sqrt(m), rounded once to 32 bits: two Newton steps in 64 from the 32-bit
 // estimate (relative error below 1e-13, far below half a step of the result),
 // a few instructions where the 64-bit root and quotient take many.
@@ -115,65 +142,72 @@ __device__ __forceinline__ float rms_factor(double m) {
   return (float)y;
 }
 
-// NC chunks per thread; chunk i of a thread is threadIdx.x + i * blockDim.x,
-// so the 16 lanes of a group are neighbours.
-template <int DT, int NC, bool NORM, bool VEC>
-__global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
+// A CTA of TPR threads (0: of any number) per row, NC chunks each: chunk i of
+// a thread is threadIdx.x + i * TPR, so the 16 lanes of a group are
+// neighbours, all but the last chunk are whole, and their places are
+// immediates. PIPE: the next row's loads are in flight while this one is
+// reduced.
+template <int DT, int TPR, int NC, bool NORM, bool VEC>
+__global__ void __launch_bounds__(TPR ? TPR : 512) k_norm_fp8(NormArgs a) {
   using E = typename Elem<DT>::T;
+  constexpr bool PIPE = NORM && TPR > 0;
   __shared__ double red[2][16];
+  const int tpr = TPR ? TPR : blockDim.x;
   const int d = a.d, chunks = (d + 7) / 8, groups = (d + FP8_BLOCK - 1) / FP8_BLOCK;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = tpr >> 5;
+  const bool last = (int)threadIdx.x + (NC - 1) * tpr < chunks;      // the last chunk is this thread's
+  const double inv_d = 1.0 / (double)d;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  Raw<DT> w[NORM ? NC : 1];
-  if constexpr (NORM)
+  Raw<DT> w[PIPE ? NC : 1];
+  if constexpr (PIPE)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      w[i] = {};
-      if (c < chunks) w[i] = load8<DT, VEC>(static_cast<const E*>(a.w), c, d);
-    }
-  int turn = 0;
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
+    for (int i = 0; i < NC; ++i)
+      w[i] = i + 1 < NC || last ? load8<DT, VEC>(static_cast<const E*>(a.w), threadIdx.x + i * tpr, d) : Raw<DT>{};
+  Raw<DT> nx[NC], nr[NORM ? NC : 1];
+  auto fetch = [&](int t) {
     const E* x = static_cast<const E*>(a.x) + t * a.x_stride;
-    Raw<DT> h[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      h[i] = {};
-      if (c < chunks) h[i] = load8<DT, VEC>(x, c, d);
-    }
-    float f = 1.f;
-    if constexpr (NORM) {
+    for (int i = 0; i < NC; ++i)
+      nx[i] = i + 1 < NC || last ? load8<DT, VEC>(x, threadIdx.x + i * tpr, d) : Raw<DT>{};
+    if constexpr (NORM)
       if (a.res) {
         const E* r = static_cast<const E*>(a.res) + t * a.res_stride;
-        Raw<DT> u[NC];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int c = threadIdx.x + i * blockDim.x;
-          if (c < chunks) u[i] = load8<DT, VEC>(r, c, d);
-        }
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int c = threadIdx.x + i * blockDim.x;
-          if (c < chunks) {
-            float p[8], q[8];
-            unpack<DT>(h[i], p);
-            unpack<DT>(u[i], q);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = __fadd_rn(p[j], q[j]);
-            h[i] = pack<DT>(p);
-            store8<DT, VEC>(static_cast<E*>(a.h) + t * a.h_stride, c, d, h[i]);
-          }
-        }
+        for (int i = 0; i < NC; ++i)
+          nr[i] = i + 1 < NC || last ? load8<DT, VEC>(r, threadIdx.x + i * tpr, d) : Raw<DT>{};
       }
-      double ss = 0.0;
+  };
+  if (PIPE && blockIdx.x < a.T) fetch(blockIdx.x);
+  int turn = 0;
+  for (int t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
+    if (!PIPE) fetch(t);
+    Raw<DT> h[NC];
+    double ss = 0.0;
+    float f = 1.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) h[i] = nx[i];
+    if constexpr (NORM) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         float v[8];
         unpack<DT>(h[i], v);
+        if (a.res) {
+          float u[8];
+          unpack<DT>(nr[i], u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fma((double)v[j], (double)v[j], ss);
+          for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(v[j], u[j]);
+          h[i] = pack<DT>(v);
+          unpack<DT>(h[i], v);
+        }
+        ss += squares(v);
+      }
+      if (PIPE && t + (int)gridDim.x < a.T) fetch(t + gridDim.x);    // h may be x or res: another row
+      if (a.res) {
+        E* o = static_cast<E*>(a.h) + t * a.h_stride;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (i + 1 < NC || last) store8<DT, VEC>(o, threadIdx.x + i * tpr, d, h[i]);
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(MS_FULL, ss, o);
@@ -181,37 +215,52 @@ __global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
         if (lane == 0) red[turn][warp] = ss;
         __syncthreads();
         ss = 0.0;
-        for (int i = 0; i < warps; ++i) ss += red[turn][i];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < warps) ss += red[turn][i];
       }
-      f = rms_factor(ss / (double)d + a.eps);
+      f = rms_factor(fma(ss, inv_d, a.eps));
     }
     uint8_t* q = a.q + t * a.q_stride;
+    float* s_row = a.s + (long long)t * groups + (threadIdx.x >> 4);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
+      const int c = threadIdx.x + i * tpr;
+      const bool mine = i + 1 < NC || last;
       float v[8], m = 0.f;
       unpack<DT>(h[i], v);
       if constexpr (NORM) {
-        float g[8];
-        unpack<DT>(w[i], g);
+        float g[8] = {};
+        if constexpr (PIPE) unpack<DT>(w[i], g);
+        else if (mine) unpack<DT>(load8<DT, VEC>(static_cast<const E*>(a.w), c, d), g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], f), g[j]);
+        for (int j = 0; j < 8; j += 2) {
+          mul2(v[j], v[j + 1], f, f);
+          mul2(v[j], v[j + 1], g[j], g[j + 1]);
+        }
       }
+      // past d: 0 times an infinite factor
+      if constexpr (VEC) {
+        m = mine ? max8_nan(v) : 0.f;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (VEC || 8 * c + j < d) m = max_nan(m, fabsf(v[j]));      // past d: 0 times an infinite factor
-      if (NORM && a.y && c < chunks) store8<DT, VEC>(static_cast<E*>(a.y) + t * a.y_stride, c, d, pack<DT>(v));
-      if (VEC && c >= chunks) m = 0.f;
+        for (int j = 0; j < 8; ++j)
+          if (8 * c + j < d) m = max_nan(m, fabsf(v[j]));
+      }
+      if (NORM && a.y && mine) store8<DT, VEC>(static_cast<E*>(a.y) + t * a.y_stride, c, d, pack<DT>(v));
 #pragma unroll
       for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(MS_FULL, m, o));
       float inv;
       const float s = group_scale(m, &inv);
-      if ((threadIdx.x & 15) == 0 && c / 16 < groups) a.s[(long long)t * groups + c / 16] = s;
-      if (c < chunks) {
+      if ((threadIdx.x & 15) == 0 && mine) s_row[i * (tpr >> 4)] = s;
+      if (mine) {
         if constexpr (VEC) {
           uint32_t b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = e4m3x2(v[2 * j] * inv, v[2 * j + 1] * inv);
+          for (int j = 0; j < 4; ++j) {
+            mul2(v[2 * j], v[2 * j + 1], inv, inv);
+            b[j] = e4m3x2(v[2 * j], v[2 * j + 1]);
+          }
           reinterpret_cast<uint2*>(q)[c] = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
         } else {
 #pragma unroll
@@ -223,10 +272,12 @@ __global__ void __launch_bounds__(512) k_norm_fp8(NormArgs a) {
   }
 }
 
-template <int DT, int NC, bool NORM, bool VEC>
-static cudaError_t launch_nc(const NormArgs& a, int threads, int grid, cudaStream_t s) {
+template <int DT, int TPR, int NC, bool NORM, bool VEC>
+static cudaError_t launch_nc(const NormArgs& a, int threads, int sms, cudaStream_t s) {
+  // PIPE: as many CTAs as are resident, so that a row's loads run ahead
+  const int per_sm = NORM && TPR ? std::max(1, 512 / threads) : 2048 / threads;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3((unsigned)std::min<long long>(a.T, (long long)per_sm * sms));
   cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -234,25 +285,35 @@ static cudaError_t launch_nc(const NormArgs& a, int threads, int grid, cudaStrea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_norm_fp8<DT, NC, NORM, VEC>, a);
+  return cudaLaunchKernelEx(&cfg, k_norm_fp8<DT, TPR, NC, NORM, VEC>, a);
+}
+
+template <int DT, int TPR, bool NORM, bool VEC>
+static cudaError_t launch_tpr(const NormArgs& a, int threads, int nc, int sms, cudaStream_t s) {
+  if (nc == 1) return launch_nc<DT, 0, 1, NORM, VEC>(a, threads, sms, s);
+  if (nc == 2) return launch_nc<DT, 0, 2, NORM, VEC>(a, threads, sms, s);
+  if (nc == 3) return launch_nc<DT, TPR, 3, NORM, VEC>(a, threads, sms, s);
+  return launch_nc<DT, TPR, 4, NORM, VEC>(a, threads, sms, s);       // 16384 features / 8 / 512
 }
 
 template <int DT, bool NORM, bool VEC>
 static cudaError_t launch_vec(const NormArgs& a, int sms, cudaStream_t s) {
-  const int chunks = (a.d + 7) / 8, whole = (chunks + 31) / 32 * 32;
-  // Rows enough to fill the GPU: three chunks a thread, so that a row's
-  // barriers and its ragged end cost little; few rows: as many threads as
-  // there are chunks.
-  const bool many = a.T >= sms * 4;
-  int nc = many ? 3 : 1;
-  while ((whole + nc - 1) / nc > 512) ++nc;
-  const int threads = std::max(32, ((chunks + nc - 1) / nc + 31) / 32 * 32);
-  const int per_sm = std::max(1, 2048 / threads);
-  const int grid = (int)std::min<long long>(a.T, (long long)sms * per_sm);
-  if (nc == 1) return launch_nc<DT, 1, NORM, VEC>(a, threads, grid, s);
-  if (nc == 2) return launch_nc<DT, 2, NORM, VEC>(a, threads, grid, s);
-  if (nc == 3) return launch_nc<DT, 3, NORM, VEC>(a, threads, grid, s);
-  return launch_nc<DT, 4, NORM, VEC>(a, threads, grid, s);      // 16384 features / 8 / 512
+  const int chunks = (a.d + 7) / 8;
+  // Rows enough to fill the GPU: three or four chunks a thread, so that a
+  // row's barrier costs little (32-bit values, twice the registers: two; 4096
+  // x 4096 35.5 us against 38.6 with four); few rows: a thread per chunk.
+  if (VEC && a.T >= sms * 4) {
+    int threads = 32;
+    while (threads < 512 && threads * (DT == DT_F32 ? 2 : 4) < chunks) threads *= 2;
+    const int nc = (chunks + threads - 1) / threads;
+    if (threads == 32) return launch_tpr<DT, 32, NORM, true>(a, 32, nc, sms, s);
+    if (threads == 64) return launch_tpr<DT, 64, NORM, true>(a, 64, nc, sms, s);
+    if (threads == 128) return launch_tpr<DT, 128, NORM, true>(a, 128, nc, sms, s);
+    if (threads == 256) return launch_tpr<DT, 256, NORM, true>(a, 256, nc, sms, s);
+    return launch_tpr<DT, 512, NORM, true>(a, 512, nc, sms, s);
+  }
+  const int nc = (chunks + 511) / 512;
+  return launch_tpr<DT, 0, NORM, VEC>(a, ((chunks + nc - 1) / nc + 31) / 32 * 32, nc, sms, s);
 }
 
 template <int DT>
