@@ -521,7 +521,7 @@ static cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s) {
       encode_fp8_map(&tx, a.x, a.K, a.M, a.x_stride, NT, 0, 0))
     return cudaErrorInvalidValue;
   auto kern = k_linear_few<NT, OUT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<NT>::SMEM);
+  cudaError_t e = allow_shared<k_linear_few<NT, OUT>>(Few<NT>::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(split, tiles, cols);
@@ -566,7 +566,7 @@ static cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t s) {
     return cudaErrorInvalidValue;
   const int y_map = encode_out_map<OUT>(&ty, a);
   auto kern = k_linear_pair<OUT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+  cudaError_t e = allow_shared<k_linear_pair<OUT>>(PAIR_SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, sms / 2) * 2);

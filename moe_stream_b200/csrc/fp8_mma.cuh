@@ -6,6 +6,8 @@
 // product is accumulated in TMEM from zero and scaled into 32-bit registers,
 // because its scale differs from the next block's.
 #pragma once
+#include <atomic>
+
 #include <cuda.h>
 
 #include "fp8.cuh"
@@ -230,6 +232,19 @@ __device__ __forceinline__ void tma_store_read_wait() {      // the source of th
 }
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Lets a kernel have `bytes` of shared memory, once per device (the attribute
+// stays; setting it again costs half a microsecond a launch).
+template <auto KERNEL>
+inline cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 
 // Codes [rows][k] with row stride `stride` bytes as 128 x box_rows tiles; with
 // mats > 0 a stack of such matrices, mat_stride bytes apart. What a tile has

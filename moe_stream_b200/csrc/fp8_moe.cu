@@ -887,7 +887,7 @@ static cudaError_t launch_experts(const MoeFp8Args& a, const MoeWs& w, int sms, 
       encode_fp8_map(&m.x, w.xq, a.d, a.T, a.d, 1, 0, 0) || encode_fp8_map(&m.h, w.hq, a.f, P, a.f, 16, 0, 0))
     return cudaErrorInvalidValue;
   auto kern = k_moe_experts<NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Moe<NT>::SMEM);
+  cudaError_t e = allow_shared<k_moe_experts<NT>>(Moe<NT>::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);

@@ -64,13 +64,14 @@ def _rows(name, t, d=None, dtype=None):
         raise TypeError(f"{name} must be a CUDA tensor")
     if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() == 0:
+    rank = t.dim()
+    if rank == 0:
         raise ValueError(f"{name} must have a feature dimension")
     n = t.shape[-1]
     if d is not None and n != d:
         raise ValueError(f"{name} has {n} features, expected {d}")
-    if t.dim() != 2:
-        t = t.reshape(-1, n) if t.numel() else t.reshape(t.numel() // n if n else 0, n)
+    if rank != 2:
+        t = t.reshape(-1, n) if t.numel() else t.reshape(0, n)
     if n > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t
@@ -99,45 +100,69 @@ def _codes_like(lead, d, device):
     return q if pad == d else q[..., :d]
 
 
+def _like(name, t, x, dev):
+    """t, a tensor that goes with x row by row, as contiguous rows."""
+    if t.get_device() != dev:
+        raise TypeError(f"{name} must be on x's device")
+    if t.dtype is not x.dtype:
+        raise TypeError(f"{name} must be {x.dtype}, got {t.dtype}")
+    if t.shape != x.shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, x {tuple(x.shape)}")
+    return t if t.is_contiguous() else _rows(name, t)
+
+
 def _norm_call(x, weight, eps, residual, h_out, with_norm):
-    if x.dtype not in _DT:
+    # A call of a few rows takes less time on the GPU than here: contiguous
+    # inputs, the ordinary case, go through with no views made of them.
+    dt = _DT.get(x.dtype)
+    if dt is None:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    x2 = _rows("x", x)
-    T, d = x2.shape
+    if x.is_contiguous() and x.is_cuda and x.dim():
+        x2, shape = x, x.shape
+        d = xs = shape[-1]
+    else:
+        x2 = _rows("x", x)
+        shape, d, xs = x.shape, x2.shape[1], _row_stride(x2)
     if not 1 <= d <= MAX_FEATURES:
         raise ValueError(f"x has {d} features, supported are 1 to {MAX_FEATURES}")
-    device, lead = x.device, x.shape[:-1]
-    dev = device.index
-    res = h = y = None
+    T = x.numel() // d
+    dev = x.get_device()
+    wp = rp = hp = yp = rs = 0
+    h = y = None
     if weight is not None:
-        if weight.dtype is not x.dtype or weight.device != device:
+        if weight.dtype is not x.dtype or weight.get_device() != dev:
             raise TypeError("weight must have x's dtype and device")
         if weight.shape != (d,):
             raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({d},)")
         if not eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
-        weight = weight.contiguous()
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        wp = weight.data_ptr()
     if residual is not None:
-        if residual.device != device:
-            raise TypeError("residual must be on x's device")
-        if residual.shape != x.shape:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
-        res = _rows("residual", residual, d, x.dtype)
-        h = torch.empty(x.shape, dtype=x.dtype, device=device) if h_out is None else \
-            _out("h_out", h_out, x.shape, x.dtype, dev)
+        res = _like("residual", residual, x, dev)
+        rp, rs = res.data_ptr(), d if res.is_contiguous() else _row_stride(res)
+        if h_out is None:
+            h = torch.empty_like(x, memory_format=torch.contiguous_format)
+        else:
+            h = _out("h_out", h_out, shape, x.dtype, dev)
+        hp = h.data_ptr()
     elif h_out is not None:
         raise ValueError("h_out needs a residual")
-    q = _codes_like(lead, d, device)
-    s = torch.empty((*lead, _blocks(d)), dtype=torch.float32, device=device)
+    if d % 16:
+        q = _codes_like(shape[:-1], d, x.device)
+    else:
+        q = torch.empty_like(x, dtype=_E4M3, memory_format=torch.contiguous_format)
+    s = x.new_empty((*shape[:-1], (d + 127) // 128), dtype=torch.float32)
     if with_norm:
-        y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        yp = y.data_ptr()
     if T:
-        args = _NORM.pack(
-            x2.data_ptr(), 0 if res is None else res.data_ptr(), 0 if weight is None else weight.data_ptr(),
-            0 if h is None else h.data_ptr(), 0 if y is None else y.data_ptr(), q.data_ptr(), s.data_ptr(),
-            _row_stride(x2), 0 if res is None else _row_stride(res), d, d, (d + 15) // 16 * 16,
-            eps, T, d, _DT[x.dtype], dev)
-        _lib.check(_lib.load().ms_rms_norm_fp8(args, _stream(dev)))
+        args = _NORM.pack(x2.data_ptr(), rp, wp, hp, yp, q.data_ptr(), s.data_ptr(),
+                          xs, rs, d, d, (d + 15) // 16 * 16, eps, T, d, dt, dev)
+        rc = _lib.load().ms_rms_norm_fp8(args, _stream(dev))
+        if rc:
+            _lib.check(rc)
     return q, s, (x if h is None else h), y
 
 
@@ -231,6 +256,7 @@ class Fp8Linear:
         self.device = w.device
         self._w = (w.data_ptr(), self.scales.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
         self._ld = _row_stride(w)
+        self._dims = (K, N, _blocks(K), w.get_device())
         self._call = _lib.load().ms_linear_fp8
 
     def __call__(self, q, scales, out_dtype=torch.bfloat16, out=None, stream=None):
@@ -241,34 +267,37 @@ class Fp8Linear:
         return self._forward(q, scales, out_dtype, out)
 
     def _forward(self, q, scales, out_dtype, out):
-        K, N = self.in_features, self.out_features
-        if q.device != self.device or scales.device != self.device:
+        K, N, KB, dev = self._dims
+        if q.get_device() != dev or scales.get_device() != dev:
             raise TypeError(f"codes and scales must be on the weight's device, {self.device}")
-        if out_dtype not in _DT:
+        dt = _DT.get(out_dtype)
+        if dt is None:
             raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
         lead = q.shape[:-1]
         if scales.shape[:-1] != lead:
             raise ValueError(f"scales have shape {tuple(scales.shape)} for codes {tuple(q.shape)}")
-        dev = self.device.index
         x = _rows("codes", q, K, _E4M3)
-        s = _rows("scales", scales, _blocks(K), torch.float32)
-        M = x.shape[0]
-        ld = x.stride(0) if M > 1 else (K + 15) // 16 * 16
+        s = _rows("scales", scales, KB, torch.float32)
+        M, ld, ls = x.shape[0], (K + 15) // 16 * 16, KB
+        if M > 1:
+            ld, ls = x.stride(0), s.stride(0)
+            if ls < KB:
+                s, ls = s.contiguous(), KB
         if x.data_ptr() % 16 or ld % 16 or ld < K:
             p = _codes_like((M,), K, x.device)
             p.copy_(x)
             x, ld = p, (K + 15) // 16 * 16
-        if M > 1 and s.stride(0) < s.shape[1]:
-            s = s.contiguous()
         if out is None:
-            out = torch.empty((*lead, N), dtype=out_dtype, device=self.device)
+            out = s.new_empty((*lead, N), dtype=out_dtype)
         else:
             _out("out", out, (*lead, N), out_dtype, dev)
         if M:
             w, ws, b = self._w
             args = _LINEAR.pack(x.data_ptr(), s.data_ptr(), w, ws, b, out.data_ptr(),
-                                ld, _row_stride(s), self._ld, N, M, N, K, _DT[out_dtype], dev, 0)
-            _lib.check(self._call(args, _stream(dev)))
+                                ld, ls, self._ld, N, M, N, K, dt, dev, 0)
+            rc = self._call(args, _stream(dev))
+            if rc:
+                _lib.check(rc)
         return out
 
 
@@ -316,6 +345,8 @@ class Fp8MoELayer:
         self._model = _lib.MODEL_GPTOSS if model == "gptoss" else _lib.MODEL_QWEN3
         lib = _lib.load()
         self._call = lib.ms_moe_fp8_layer
+        self._dev = self.router.get_device()
+        self._tail = (self.d_model, self.d_ff, self.n_experts, self.top_k, self.norm_topk_prob, self._dev)
         self._ws = [0] * (MAX_TOKENS + 1)
         n = ctypes.c_size_t()
         for T in range(1, MAX_TOKENS + 1):
@@ -324,13 +355,12 @@ class Fp8MoELayer:
 
     @staticmethod
     def _aligned(t):
-        t = t.contiguous()
+        if not t.is_contiguous():
+            t = t.contiguous()
         return t.clone() if t.data_ptr() % 16 else t
 
     def _pack(self, x, residual, y, ws, ws_bytes, T):
-        return _MOE.pack(x, *self._router, *self._ptrs, residual, y, ws, ws_bytes, self._model, T,
-                         self.d_model, self.d_ff, self.n_experts, self.top_k, self.norm_topk_prob,
-                         self.device.index)
+        return _MOE.pack(x, *self._router, *self._ptrs, residual, y, ws, ws_bytes, self._model, T, *self._tail)
 
     def __call__(self, x, residual=None, out=None, stream=None):
         """x [..., d] bf16 -> y [..., d] bf16, residual (like x) added. out
@@ -340,30 +370,29 @@ class Fp8MoELayer:
         return self._forward(x, residual, out)
 
     def _forward(self, x, residual, out):
-        d, dev = self.d_model, self.device
-        if x.device != dev:
-            raise TypeError(f"x must be on the layer's device, {dev}")
-        x2 = self._aligned(_rows("x", x, d, torch.bfloat16))
+        d, dev = self.d_model, self._dev
+        if x.get_device() != dev:
+            raise TypeError(f"x must be on the layer's device, {self.device}")
+        x2 = _rows("x", x, d, torch.bfloat16)
+        if not x2.is_contiguous() or x2.data_ptr() % 16:
+            x2 = self._aligned(x2)
         T = x2.shape[0]
         if T > MAX_TOKENS:
             raise ValueError(f"{T} tokens, at most {MAX_TOKENS} per call")
-        r2 = None
+        rp = 0
         if residual is not None:
-            if residual.device != dev:
-                raise TypeError(f"residual must be on the layer's device, {dev}")
-            if residual.shape != x.shape:
-                raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
-            r2 = self._aligned(_rows("residual", residual, d, torch.bfloat16))
+            r2 = self._aligned(_like("residual", residual, x, dev))
+            rp = r2.data_ptr()
         if out is None:
-            out = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
-            _out("out", out, x.shape, torch.bfloat16, dev.index)
+            _out("out", out, x.shape, torch.bfloat16, dev)
             if out.data_ptr() % 16:
                 raise ValueError("out must start on a 16-byte boundary")
         if T:
             nb = self._ws[T]
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-            _lib.check(self._call(
-                self._pack(x2.data_ptr(), 0 if r2 is None else r2.data_ptr(), out.data_ptr(),
-                           ws.data_ptr(), nb, T), _stream(dev.index)))
+            ws = x.new_empty(nb, dtype=torch.uint8)
+            rc = self._call(self._pack(x2.data_ptr(), rp, out.data_ptr(), ws.data_ptr(), nb, T), _stream(dev))
+            if rc:
+                _lib.check(rc)
         return out
