@@ -134,6 +134,13 @@ __device__ __forceinline__ void tmem_wait16(uint32_t* r) {
                : "memory");
 }
 
+// one column, here when it returns
+__device__ __forceinline__ float tmem_read1(uint32_t t) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(t));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r) : : "memory");
+  return __uint_as_float(r);
+}
 // 32 consecutive columns; tmem_wait32 before use
 __device__ __forceinline__ void tmem_load32(uint32_t t, uint32_t* r) {
   asm volatile(

@@ -36,6 +36,12 @@
 // pipeline serves both: a step is two 128 x 128 weight tiles, an up task's gate
 // and up tile of one block or a down task's tiles of two blocks (of one, where
 // the expert has more than 16 rows).
+//
+// A single token (ONE) hands its sums and codes on as 8-byte words of a value
+// and a mark, which k_moe_route has cleared: the reader polls the word itself.
+// Handing on by a flag costs two trips more, a fence before the flag and a
+// load after it, and one token's layer is a chain of such trips (LLTIMES).
+//
 // Warps 0-3 and 8-11 take products out of TMEM and do the rest of a task, two
 // groups with a task each, so that one's end overlaps the other's products;
 // warp 4 loads weights and takes tasks, warp 5 issues MMAs, warp 6 loads
@@ -90,27 +96,64 @@ struct MoeWs {            // workspace layout
   unsigned* dn_done;      // [tile of d] down tasks done
   int counters;           // words from next on
   int cap1, cap2;         // split_cap of the up and down tiles
+  // one token: words of a value and a mark, zeroed by k_moe_route
+  unsigned long long* up_w;   // [S1 - 1][2][k][f]
+  unsigned long long* h_w;    // [k][f / 4] four codes each
+  unsigned long long* hs_w;   // [k][blocks of f]
+  unsigned long long* dn_w;   // [S2][k][d]
+  long long words;        // of all of them
+  int S1, S2;             // ranges of its tiles
 };
 
-static long long layout_ws(uint8_t* w, int T, int d, int f, int E, int k, MoeWs* o) {
+// Ranges for n tiles of kb blocks on `ctas` CTAs are the number with the least
+// (rounds of tasks, half a round for the ragged end) x (blocks of a task, half
+// a block for its end and `join` for sums that have to meet). In blocks: a
+// Qwen3 up tile's join was about two of its blocks long.
+__host__ __device__ inline float split_cost(int s, int n, int kb, int ctas, float join) {
+  float rounds = (float)(n * s) / (float)ctas;
+  rounds = rounds <= 1.f ? 1.f : rounds + 0.5f;
+  return rounds * ((float)((kb + s - 1) / s) + 0.5f + (s > 1 ? join : 0.f));
+}
+static int best_split(int n, int kb, int ctas, int cap, float join) {
+  int best = (kb + MOE_FAC - 1) / MOE_FAC;
+  for (int s = best + 1; s <= cap && s <= kb; ++s)
+    if (split_cost(s, n, kb, ctas, join) < split_cost(best, n, kb, ctas, join)) best = s;
+  return best;
+}
+
+static long long layout_ws(uint8_t* w, int T, int d, int f, int E, int k, int ctas, MoeWs* o) {
   const long long P = (long long)T * k;
   const int tiles = (int)std::min<long long>(P, E) * blocks128(f);
-  uint8_t* const w0 = w;
+  uint8_t* const base = w;
+  *o = MoeWs{};
   o->cap1 = split_cap(2 * P, f, blocks128(d)), o->cap2 = split_cap(P, d, blocks128(f));
   o->xq = w, w += up16((long long)T * d);
   o->hq = w, w += up16(P * f);
   o->logits = reinterpret_cast<float*>(w), w += up16(4ll * T * E);
   o->xs = reinterpret_cast<float*>(w), w += up16(4ll * T * blocks128(d));
   o->hs = reinterpret_cast<float*>(w), w += up16(4 * P * blocks128(f));
-  o->up_part = reinterpret_cast<float*>(w), w += 8ll * o->cap1 * P * f;
-  o->dn_part = reinterpret_cast<float*>(w), w += 4ll * o->cap2 * P * d;
+  o->up_part = o->dn_part = nullptr;
+  if (T == 1) {
+    const int FT = blocks128(f), DT = blocks128(d);
+    o->S1 = best_split(k * FT, DT, ctas, MOE_SPLIT, 1.f), o->S2 = best_split(k * DT, FT, ctas, MOE_SPLIT, 0.5f);
+    const auto w0 = reinterpret_cast<unsigned long long*>(w);
+    o->h_w = w0, o->hs_w = o->h_w + (long long)k * f / 4;
+    o->dn_w = o->hs_w + (k * FT + 1) / 2 * 2, o->up_w = o->dn_w + (long long)o->S2 * k * d;
+    o->words = o->up_w + (o->S1 - 1) * 2ll * k * f - w0;
+    // room for any number of CTAs
+    w += 8 * ((long long)k * f / 4 + k * FT + 1 + (long long)MOE_SPLIT * k * d + (MOE_SPLIT - 1) * 2ll * k * f);
+    w += (16 - (w - base) % 16) % 16;
+  } else {
+    o->up_part = reinterpret_cast<float*>(w), w += 8ll * o->cap1 * P * f;
+    o->dn_part = reinterpret_cast<float*>(w), w += 4ll * o->cap2 * P * d;
+  }
   o->inds = reinterpret_cast<int*>(w), w += up16(4 * P);
   o->probs = reinterpret_cast<float*>(w), w += up16(4 * P);
   o->next = reinterpret_cast<unsigned*>(w), o->rt_next = o->next + 1, o->routed = o->next + 2;
   o->brought = o->next + 3, o->flag = o->brought + tiles, o->dn_done = o->flag + tiles;
   o->counters = 3 + 2 * tiles + blocks128(d);
   w += up16(4ll * o->counters);
-  return w - w0;
+  return w - base;
 }
 
 // --------------------------------------------------------------------- route
@@ -156,6 +199,9 @@ __global__ void __launch_bounds__(256) k_moe_route(MoeFp8Args a, MoeWs w) {
   const int q = blockIdx.x - ex, nq = gridDim.x - ex;          // q-th of the quantising CTAs of this row
   if (blockIdx.y == 0 && q == 0)
     for (int i = threadIdx.x; i < w.counters; i += 256) w.next[i] = 0;
+  if (TG == 1)
+    for (long long i = q * 256 + threadIdx.x; i < w.words / 2; i += nq * 256)
+      reinterpret_cast<uint4*>(w.h_w)[i] = make_uint4(0, 0, 0, 0);
   const int groups = blocks128(a.d);
   // a half-warp per group of 128 features
   for (int i = (blockIdx.y * nq + q) * 16 + warp * 2 + (lane >> 4); i < a.T * groups; i += gridDim.y * nq * 16) {
@@ -237,19 +283,70 @@ struct Shape {            // what the tasks are
   }
 };
 
-// Ranges for n tiles of kb blocks on `ctas` CTAs, by a warp (a number per
-// lane): the least (rounds of tasks, half a round for the ragged end) x
-// (blocks of a task, half a block for its end and `join` for sums that have to
-// meet). In blocks: a Qwen3 up tile's join was about two of its blocks long.
+// The best number of ranges, by a warp (a number per lane).
 __device__ __forceinline__ int choose_split(int n, int kb, int ctas, int cap, float join) {
   const int s = (threadIdx.x & 31) + 1;
-  float rounds = (float)(n * s) / (float)ctas;
-  rounds = rounds <= 1.f ? 1.f : rounds + 0.5f;
-  const float cost = rounds * ((float)((kb + s - 1) / s) + 0.5f + (s > 1 ? join : 0.f));
   const bool can = s >= (kb + MOE_FAC - 1) / MOE_FAC && s <= cap && s <= kb;
-  const unsigned key = can ? __float_as_uint(cost) : 0x7f800000u;
+  const unsigned key = can ? __float_as_uint(split_cost(s, n, kb, ctas, join)) : 0x7f800000u;
   const unsigned least = __reduce_min_sync(MS_FULL, key);
   return __ffs(__ballot_sync(MS_FULL, key == least));
+}
+
+// A value and its mark in one word, written and read whole.
+__device__ __forceinline__ void put_word(unsigned long long* p, uint32_t v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(1ull << 32 | v) : "memory");
+}
+__device__ __forceinline__ unsigned long long get_word(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+// v[q] = the value of word p[q * stride] for q < n, once all are written; a
+// second at most.
+// Four words from each of four places, as wait_words.
+__device__ __forceinline__ void wait_quads(const unsigned long long* const* p, uint32_t (*v)[4]) {
+  unsigned long long t0 = 0;
+  for (unsigned i = 0;; ++i) {
+    unsigned have = 0;
+    unsigned long long x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[j][q] = get_word(p[j] + q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[j][q] = (uint32_t)x[j][q], have += (unsigned)(x[j][q] >> 32);
+    if (have == 16) return;
+    if ((i & 63) == 63) {
+      const unsigned long long now = global_ns();
+      if (!t0) t0 = now;
+      if (now - t0 > MBAR_WAIT_NS || timed_out(&g_moe_status)) break;
+    }
+  }
+  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
+}
+template <int N>
+__device__ __forceinline__ void wait_words(const unsigned long long* p, long long stride, int n, uint32_t* v) {
+  unsigned long long t0 = 0;
+  unsigned have = 0;
+  for (unsigned i = 0;; ++i) {
+    unsigned long long x[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (q < n) x[q] = get_word(p + q * stride);
+    have = 0;
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (q < n) v[q] = (uint32_t)x[q], have += (unsigned)(x[q] >> 32);
+    if (have == (unsigned)n) return;
+    if ((i & 63) == 63) {
+      const unsigned long long now = global_ns();
+      if (!t0) t0 = now;
+      if (now - t0 > MBAR_WAIT_NS || timed_out(&g_moe_status)) break;
+    }
+  }
+  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
 }
 
 __device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
@@ -312,7 +409,7 @@ struct MoeMaps {
   CUtensorMap gate, up, down, x, h;
 };
 
-template <int NT>
+template <int NT, bool ONE>
 __global__ void __launch_bounds__(MOE_THREADS, 1)
     k_moe_experts(const __grid_constant__ MoeMaps maps, const __grid_constant__ MoeFp8Args a,
                   const __grid_constant__ MoeWs w) {
@@ -455,7 +552,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       s_group[(at >> 16) - 1] = (uint8_t)threadIdx.x;
       s_start[threadIdx.x] = (at & 0xffff) - mine_n;
     }
-  } else if (warp < 10) {
+  } else if (!ONE && warp < 10) {
     const int nf = blocks128(a.f), nd = blocks128(a.d);
     const int split = warp == 8 ? choose_split(G * nf, nd, gridDim.x, w.cap1, 2.f)
                                 : choose_split(G * nd, nf, gridDim.x, w.cap2, 0.5f);
@@ -470,7 +567,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   }
   __syncthreads();
   Shape sh;
-  sh.G = G, sh.S1 = s_word[4], sh.S2 = s_word[5];
+  sh.G = G, sh.S1 = ONE ? w.S1 : s_word[4], sh.S2 = ONE ? w.S2 : s_word[5];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
   sh.n_up = sh.G * sh.FT * sh.S1, sh.n_dn = sh.G * sh.DT * sh.S2;
   sh.n_co = sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
@@ -591,6 +688,34 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (t.kind == 2) continue;
       const int e = s_group[t.g], start = s_start[e], rows = __popcll(s_mask[e]);
       const int per = t.kind == 0 ? 1 : down_per(t.g);
+      if constexpr (ONE)
+        if (t.kind == 1) {
+          // the row's codes, word by word, into the first row of the tiles
+          const int n4 = a.f / 4;
+          uint32_t v[MOE_FAC];
+#pragma unroll
+          for (int q = 0; q < MOE_FAC; ++q) v[q] = 0;
+          // a lane's last block may lie beyond f
+          const int at0 = t.b0 * 32 + lane, nb = t.b1 - t.b0 - (at0 + (t.b1 - t.b0 - 1) * 32 >= n4);
+          wait_words<MOE_FAC>(w.h_w + (long long)start * n4 + at0, 32, nb, v);
+#pragma unroll
+          for (int q = 0; q < MOE_FAC; q += 2) {
+            if (t.b0 + q >= t.b1) break;
+            const int s = i % C::STAGES;
+            if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
+              ok = false;
+              break;
+            }
+            uint8_t* at = smem + s * C::STAGE + 2 * FP8_W_TILE + 4 * lane;
+            *reinterpret_cast<uint32_t*>(at) = q < nb ? v[q] : 0;
+            *reinterpret_cast<uint32_t*>(at + 2048) = q + 1 < nb ? v[q + 1] : 0;
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&full[s]);
+            ++i;
+          }
+          continue;
+        }
       int tok[4];                            // up: the tokens of rows 4 lane to 4 lane + 3, none beyond the last
       if (t.kind == 1) {
         for (int b = t.b0 + lane; b < t.b1; b += 32) wait_count(w.flag + t.g * sh.FT + b, 1);
@@ -648,6 +773,17 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
       } else {
         const float wd = __ldg(a.down.s + ((long long)e * sh.DT + t.tile) * sh.KB2 + b);
+        if constexpr (ONE) {
+          uint32_t x;
+          wait_words<1>(w.hs_w + (long long)start * sh.KB2 + b, 0, 1, &x);
+          __syncwarp();
+          if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
+          if (lane < nb) fac[0] = __uint_as_float(x) * wd;
+          ++c;
+          __syncwarp();
+          if (lane == 0) mbar_arrive1(&f_full[u]);
+          continue;
+        }
         wait_count(w.flag + t.g * sh.FT + b, 1);
         __syncwarp();
         if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
@@ -688,8 +824,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         if (!combine) continue;
         // y of four tokens, one per warp: rows in the order of the token's
         // choices, ranges in order
-        if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2));
-        meet();
+        if (!ONE) {
+          if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2));
+          meet();
+        }
         const int f = t.tile * 128 + lane * 4, tok = t.s * COMBINE_T + warp;
         if (f < a.d && tok < a.T) {
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -700,6 +838,23 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
             for (int j = 0; j < 8; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int s = 0; s < sh.S2; ++s) {
               const int r0 = s * P;
+              if constexpr (ONE) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {       // four choices' words in flight
+                  const unsigned long long* p[4];
+                  uint32_t v[4][4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    p[j] = w.dn_w + (long long)(r0 + s_row[min(j0 + 4 * h + j, a.k - 1)]) * a.d + f;
+                  wait_quads(p, v);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    o[4 * h + j].x += __uint_as_float(v[j][0]), o[4 * h + j].y += __uint_as_float(v[j][1]);
+                    o[4 * h + j].z += __uint_as_float(v[j][2]), o[4 * h + j].w += __uint_as_float(v[j][3]);
+                  }
+                }
+                continue;
+              }
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const int row = r0 + s_row[tok * 32 + min(j0 + j, a.k - 1)];
@@ -741,6 +896,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
 #pragma unroll
       for (int m = 0; m < NT; ++m) acc[0][m] = acc[1][m] = 0.f;
       auto take = [&](float* sum, uint32_t at, const float* f) {
+        if constexpr (ONE) {
+          sum[0] = fmaf(tmem_read1(at), f[0], sum[0]);
+          return;
+        }
 #pragma unroll
         for (int m = 0; m < NT; m += 16) {
           if (m >= rows) break;
@@ -782,6 +941,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (t.kind == 1) {
         float* part = w.dn_part + (t.s * (long long)P + start) * a.d + f;
         const float bias = t.s == 0 && a.down.bias && f < a.d ? __ldg(a.down.bias + (long long)e * a.d + f) : 0.f;
+        if constexpr (ONE) {
+          if (f < a.d) put_word(w.dn_w + (long long)(t.s * P + start) * a.d + f, __float_as_uint(acc[0][0] + bias));
+          continue;
+        }
         if (f < a.d)
 #pragma unroll
           for (int m = 0; m < NT; ++m)
@@ -791,7 +954,26 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         continue;
       }
       const int tile = t.g * sh.FT + t.tile;
-      if (sh.S1 > 1) {
+      if constexpr (ONE) {
+        // the last range's CTA adds the others' sums to its own
+        if (f < a.f) {
+          unsigned long long* word = w.up_w + (long long)start * a.f + f;
+          const long long stride = (long long)a.k * a.f;
+          if (t.s < sh.S1 - 1) {
+            put_word(word + 2 * t.s * stride, __float_as_uint(acc[0][0]));
+            put_word(word + (2 * t.s + 1) * stride, __float_as_uint(acc[1][0]));
+          } else if (sh.S1 > 1) {
+            uint32_t v[2 * (MOE_SPLIT - 1)];
+            wait_words<2 * (MOE_SPLIT - 1)>(word, stride, 2 * (sh.S1 - 1), v);
+            float g = 0.f, u = 0.f;
+#pragma unroll
+            for (int q = 0; q < MOE_SPLIT - 1; ++q)
+              if (q < sh.S1 - 1) g += __uint_as_float(v[2 * q]), u += __uint_as_float(v[2 * q + 1]);
+            acc[0][0] += g, acc[1][0] += u;
+          }
+        }
+        if (t.s < sh.S1 - 1) continue;
+      } else if (sh.S1 > 1) {
         if (f < a.f) {
           float* pg = w.up_part + (t.s * 2ll * P + start) * a.f + f;
           float* pu = pg + (long long)P * a.f;
@@ -820,7 +1002,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
           if (a.up.bias) bu[q] = __ldg(a.up.bias + (long long)e * a.f + f4 + q);
         }
       for (int r0 = 0; r0 < rows; r0 += MOE_ROWS) {
-        if (sh.S1 == 1) {                    // this tile's sums are in the registers of their columns
+        if (ONE || sh.S1 == 1) {             // this tile's sums are in the registers of their columns
 #pragma unroll
           for (int m = 0; m < NT; m += MOE_ROWS)
             if (m == r0) {
@@ -834,7 +1016,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
         for (int r = r0 + (warp & 3); r < min(rows, r0 + MOE_ROWS); r += 4) {
           float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
-          if (sh.S1 == 1) {
+          if (ONE || sh.S1 == 1) {
             g = *reinterpret_cast<const float4*>(s_rows + (r - r0) * 128 + lane * 4);
             u = *reinterpret_cast<const float4*>(s_rows + (MOE_ROWS + r - r0) * 128 + lane * 4);
           } else if (in) {
@@ -854,13 +1036,18 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
           float inv;
           const float s = group_scale(
               warp_max(max_nan(max_nan(fabsf(h0), fabsf(h1)), max_nan(fabsf(h2), fabsf(h3)))), &inv);
-          if (in)
-            *reinterpret_cast<uint32_t*>(w.hq + (long long)(start + r) * a.f + f4) =
-                e4m3x2(h0 * inv, h1 * inv) | e4m3x2(h2 * inv, h3 * inv) << 16;
+          const uint32_t codes = e4m3x2(h0 * inv, h1 * inv) | e4m3x2(h2 * inv, h3 * inv) << 16;
+          if constexpr (ONE) {
+            if (in) put_word(w.h_w + ((long long)(start + r) * a.f + f4) / 4, codes);
+            if (lane == 0) put_word(w.hs_w + (long long)(start + r) * sh.KB2 + t.tile, __float_as_uint(s));
+            continue;
+          }
+          if (in) *reinterpret_cast<uint32_t*>(w.hq + (long long)(start + r) * a.f + f4) = codes;
           if (lane == 0) w.hs[(long long)(start + r) * sh.KB2 + t.tile] = s;
         }
-        if (sh.S1 == 1) meet(); // the rows have been read
+        if (ONE || sh.S1 == 1) meet();       // the rows have been read
       }
+      if (ONE) continue;
       fence_async_all();                     // the codes are read by tensor copies
       meet();
       if (tid == 0) red_release(w.flag + tile);
@@ -874,10 +1061,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
 // ------------------------------------------------------------------ launches
 size_t moe_fp8_workspace(int T, int d, int f, int E, int k) {
   MoeWs w;
-  return (size_t)layout_ws(nullptr, T, d, f, E, k, &w);
+  return (size_t)layout_ws(nullptr, T, d, f, E, k, 148, &w);
 }
 
-template <int NT>
+template <int NT, bool ONE>
 static cudaError_t launch_experts(const MoeFp8Args& a, const MoeWs& w, int sms, cudaStream_t s) {
   const long long P = (long long)a.T * a.k, ew = (long long)a.d * a.f;
   MoeMaps m;
@@ -886,8 +1073,8 @@ static cudaError_t launch_experts(const MoeFp8Args& a, const MoeWs& w, int sms, 
       encode_fp8_map(&m.down, a.down.q, a.f, a.d, a.f, 128, a.E, ew) ||
       encode_fp8_map(&m.x, w.xq, a.d, a.T, a.d, 1, 0, 0) || encode_fp8_map(&m.h, w.hq, a.f, P, a.f, 16, 0, 0))
     return cudaErrorInvalidValue;
-  auto kern = k_moe_experts<NT>;
-  cudaError_t e = allow_shared<k_moe_experts<NT>>(Moe<NT>::SMEM);
+  auto kern = k_moe_experts<NT, ONE>;
+  cudaError_t e = allow_shared<k_moe_experts<NT, ONE>>(Moe<NT>::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);
@@ -906,8 +1093,9 @@ template <int TG>
 static cudaError_t launch_route(const MoeFp8Args& a, const MoeWs& w, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   const int rows = (a.T + TG - 1) / TG;
-  // a quantising CTA per 16 groups of its share of the tokens
-  cfg.gridDim = dim3((a.E + 7) / 8 + std::max(1, (TG * blocks128(a.d) + 15) / 16), rows);
+  // a quantising CTA per 16 groups of its share of the tokens, or per 16 KB to clear
+  const int clear = TG == 1 ? (int)std::min<long long>(64, (w.words + 2047) / 2048) : 1;
+  cfg.gridDim = dim3((a.E + 7) / 8 + std::max(clear, (TG * blocks128(a.d) + 15) / 16), rows);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -920,12 +1108,13 @@ static cudaError_t launch_route(const MoeFp8Args& a, const MoeWs& w, cudaStream_
 
 cudaError_t launch_moe_fp8(const MoeFp8Args& a, int sms, cudaStream_t s) {
   MoeWs w;
-  layout_ws(a.ws, a.T, a.d, a.f, a.E, a.k, &w);
+  layout_ws(a.ws, a.T, a.d, a.f, a.E, a.k, sms, &w);
   cudaError_t e = a.T == 1 ? launch_route<1>(a, w, s) : a.T <= 16 ? launch_route<4>(a, w, s) : launch_route<8>(a, w, s);
   if (e != cudaSuccess) return e;
-  if (a.T <= 16) return launch_experts<16>(a, w, sms, s);
-  if (a.T <= 32) return launch_experts<32>(a, w, sms, s);
-  return launch_experts<64>(a, w, sms, s);
+  if (a.T == 1) return launch_experts<16, true>(a, w, sms, s);
+  if (a.T <= 16) return launch_experts<16, false>(a, w, sms, s);
+  if (a.T <= 32) return launch_experts<32, false>(a, w, sms, s);
+  return launch_experts<64, false>(a, w, sms, s);
 }
 
 cudaError_t moe_fp8_status(int** at) { return cudaGetSymbolAddress(reinterpret_cast<void**>(at), g_moe_status); }

@@ -319,7 +319,10 @@ def check_moe(y, x, router, rb, parts, k, model, norm=True, res=None):
     ("qwen3", 64, 384, 128, 1, 1), ("qwen3", 2, 256, 256, 256, 32), ("gptoss", 64, 128, 128, 256, 32),
     # many tasks on every SM, tiles cut into ranges by their length
     ("qwen3", 16, 2048, 768, 128, 8), ("gptoss", 5, 2880, 1440, 32, 4), ("qwen3", 61, 1024, 512, 64, 8),
-    ("qwen3", 30, 2880, 2880, 4, 2)])
+    ("qwen3", 30, 2880, 2880, 4, 2),
+    # single tokens: one block, ragged blocks, one expert, many
+    ("qwen3", 1, 128, 128, 4, 1), ("gptoss", 1, 272, 144, 16, 4), ("gptoss", 1, 2880, 2880, 4, 4),
+    ("qwen3", 1, 400, 656, 256, 32), ("qwen3", 1, 2048, 768, 128, 8), ("gptoss", 1, 4112, 1040, 2, 1)])
 def test_moe(model, T, d, f, E, k, lib, cuda):
     g = _gen(T + d + f + E)
     layer, router, rb, parts = make_moe(g, model, d, f, E, k)
