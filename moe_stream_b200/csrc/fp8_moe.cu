@@ -405,6 +405,61 @@ __device__ __forceinline__ bool wait_count(const unsigned* p, unsigned want) {
   return false;
 }
 
+// A token's experts: lane j holds the j-th choice and its key.
+struct Choice {
+  int expert;
+  uint32_t key;
+  float top, all;           // largest logit (NaN where one is); sum over all experts, if it is asked for
+};
+// The largest logit one after another. The code runs once, cold, so it is
+// kept short.
+__device__ __forceinline__ Choice choose(const float* logits, const MoeFp8Args& a, int lane) {
+  uint32_t key[8];
+  float v[8];
+  bool nan = false;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < a.E ? __ldcg(logits + e) + 0.f : 0.f;      // -0 is 0
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    nan |= v[i] != v[i];
+    key[i] = lane + 32 * i < a.E ? order_key(v[i]) : 0u;
+    top = max(top, key[i]);
+  }
+  Choice c{0, 0u, 0.f, 0.f};
+  const float m = key_value(__reduce_max_sync(MS_FULL, top));
+  c.top = __any_sync(MS_FULL, nan) ? __uint_as_float(0x7fc00000u) : m;
+  if (a.model == 0 && !a.norm_topk) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c.all += lane + 32 * i < a.E ? expf(v[i] - c.top) : 0.f;
+    c.all = warp_sum(c.all);
+  }
+  for (int j = 0; j < a.k; ++j) {
+    const uint32_t b0 = max(max(key[0], key[1]), max(key[2], key[3]));
+    const uint32_t b1 = max(max(key[4], key[5]), max(key[6], key[7]));
+    const uint32_t best = __reduce_max_sync(MS_FULL, max(b0, b1));
+    int e = 1 << 20;
+#pragma unroll
+    for (int i = 7; i >= 0; --i)
+      if (key[i] == best) e = lane + 32 * i;
+    const int first = __reduce_min_sync(MS_FULL, e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i == first) key[i] = 0;
+    if (lane == j) c.expert = first, c.key = best;
+  }
+  return c;
+}
+// lane j: the j-th choice's share
+__device__ __forceinline__ float share(const Choice& c, const MoeFp8Args& a, int lane) {
+  const float p = lane < a.k ? expf(key_value(c.key) - c.top) : 0.f;
+  const float sel = warp_sum(p);
+  return p / (a.model == 1 || a.norm_topk ? sel : c.all);
+}
+
 struct MoeMaps {
   CUtensorMap gate, up, down, x, h;
 };
@@ -458,72 +513,52 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   unsigned first_task = 0;
   if (warp == 4 && lane == 0) first_task = atomicAdd(w.next, 1u);    // back by the time it can be read
 
-  // ---- the routing: a warp per token takes the largest logit one after
-  // another. The code runs once, cold, so it is kept short.
-  const bool shared_out = a.T > MOE_THREADS / 32;
-  if (!shared_out || warp == 0)
+  // ---- the routing, a warp per token
+  const bool shared_out = !ONE && a.T > MOE_THREADS / 32;
+  int G = a.k;
+  if constexpr (ONE) {
+    Choice c;
+    if (warp == 0) {
+      c = choose(w.logits, a, lane);
+      int rank = 0;                         // rows lie in the order of their experts
+      for (int j = 0; j < a.k; ++j) rank += __shfl_sync(MS_FULL, c.expert, j) < c.expert;
+      if (lane < a.k) {
+        s_group[rank] = (uint8_t)c.expert;
+        s_start[c.expert] = rank;
+        s_mask[c.expert] = 1;
+        s_row[lane] = (uint16_t)rank;
+        s_tok[rank] = 0;
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {                        // read by this warp alone, at the end
+      const float p = share(c, a, lane);
+      if (lane < a.k) s_prob[lane] = p;
+    }
+  } else if (!shared_out || warp == 0) {
     for (int t = warp;; t = a.T) {
       if (shared_out) {
         if (lane == 0) t = (int)atomicAdd(w.rt_next, 1u);
         t = __shfl_sync(MS_FULL, t, 0);
       }
       if (t >= a.T) break;
-      uint32_t key[8];
-      float v[8];
-      bool nan = false;
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = lane + 32 * i;
-        v[i] = e < a.E ? __ldcg(w.logits + t * a.E + e) + 0.f : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        nan |= v[i] != v[i];
-        key[i] = lane + 32 * i < a.E ? order_key(v[i]) : 0u;
-        top = max(top, key[i]);
-      }
-      const float m0 = key_value(__reduce_max_sync(MS_FULL, top));
-      const float m = __any_sync(MS_FULL, nan) ? __uint_as_float(0x7fc00000u) : m0;
-      uint32_t mine_key = 0;                  // lane j: the j-th choice
-      int mine = 0;
-      float all = 0.f;
-      if (a.model == 0 && !a.norm_topk) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) all += lane + 32 * i < a.E ? expf(v[i] - m) : 0.f;
-        all = warp_sum(all);
-      }
-      for (int j = 0; j < a.k; ++j) {
-        const uint32_t b0 = max(max(key[0], key[1]), max(key[2], key[3]));
-        const uint32_t b1 = max(max(key[4], key[5]), max(key[6], key[7]));
-        const uint32_t best = __reduce_max_sync(MS_FULL, max(b0, b1));
-        int e = 1 << 20;
-#pragma unroll
-        for (int i = 7; i >= 0; --i)
-          if (key[i] == best) e = lane + 32 * i;
-        const int first = __reduce_min_sync(MS_FULL, e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (lane + 32 * i == first) key[i] = 0;
-        if (lane == j) mine = first, mine_key = best;
-      }
-      const float p = lane < a.k ? expf(key_value(mine_key) - m) : 0.f;
-      const float sel = warp_sum(p);
+      const Choice c = choose(w.logits + t * a.E, a, lane);
+      const float p = share(c, a, lane);
       if (lane < a.k) {
-        const float share = p / (a.model == 1 || a.norm_topk ? sel : all);
         if (shared_out) {
-          __stcg(w.probs + t * a.k + lane, share);
-          __stcg(w.inds + t * a.k + lane, mine);
+          __stcg(w.probs + t * a.k + lane, p);
+          __stcg(w.inds + t * a.k + lane, c.expert);
         } else {
-          s_prob[t * 32 + lane] = share;
-          s_row[t * 32 + lane] = (uint16_t)mine;
-          atomicOr(&s_mask[mine], 1ull << t);
+          s_prob[t * 32 + lane] = p;
+          s_row[t * 32 + lane] = (uint16_t)c.expert;
+          atomicOr(&s_mask[c.expert], 1ull << t);
         }
       }
       __syncwarp();
       if (shared_out && lane == 0) red_release(w.routed);
       if (!shared_out) break;
     }
+  }
   if (shared_out) {
     if (threadIdx.x == 0) wait_count(w.routed, (unsigned)a.T);
     __syncthreads();
@@ -534,10 +569,11 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       atomicOr(&s_mask[e], 1ull << t);
     }
   }
+  if constexpr (!ONE) {
   __syncthreads();
   // groups: the experts that have rows, ascending; their rows follow each other
   const int mine_n = threadIdx.x < 256 ? __popcll(s_mask[threadIdx.x]) : 0;
-  const int G = __syncthreads_count(mine_n > 0);
+  G = __syncthreads_count(mine_n > 0);
   if (warp < 8) {                           // rows in the low half, groups in the high; sums of the warps before
     int at = mine_n + (mine_n ? 1 << 16 : 0);
 #pragma unroll
@@ -552,7 +588,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       s_group[(at >> 16) - 1] = (uint8_t)threadIdx.x;
       s_start[threadIdx.x] = (at & 0xffff) - mine_n;
     }
-  } else if (!ONE && warp < 10) {
+  } else if (warp < 10) {
     const int nf = blocks128(a.f), nd = blocks128(a.d);
     const int split = warp == 8 ? choose_split(G * nf, nd, gridDim.x, w.cap1, 2.f)
                                 : choose_split(G * nd, nf, gridDim.x, w.cap2, 0.5f);
@@ -566,6 +602,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     s_tok[row] = (uint8_t)t;
   }
   __syncthreads();
+  }
   Shape sh;
   sh.G = G, sh.S1 = ONE ? w.S1 : s_word[4], sh.S2 = ONE ? w.S2 : s_word[5];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
