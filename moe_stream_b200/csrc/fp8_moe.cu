@@ -157,24 +157,28 @@ static long long layout_ws(uint8_t* w, int T, int d, int f, int E, int k, int ct
 }
 
 // --------------------------------------------------------------------- route
-// A warp per expert and TG tokens; the CTAs after the experts' quantise x, a
-// warp per token, and zero the counters.
+// Four warps per expert and TG tokens, two experts a CTA, so that all loads of
+// a warp are in flight at once; the CTAs after the experts' quantise x and
+// clear the counters.
 template <int TG>
 __global__ void __launch_bounds__(256) k_moe_route(MoeFp8Args a, MoeWs w) {
+  __shared__ float part[8][TG];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int chunks = a.d / 8, ex = (a.E + 7) / 8;
+  const int chunks = a.d / 8, ex = (a.E + 1) / 2;
+  const int e = min((int)blockIdx.x * 2 + (warp >> 2), a.E - 1), c0 = (warp & 3) * 32 + lane;
+  const uint4* wr = reinterpret_cast<const uint4*>(a.router + (long long)e * a.d);
+  if ((int)blockIdx.x < ex)                  // into L2 alone: it may run ahead of what wrote it
+    for (int c = c0; c < chunks; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(wr + c));
   grid_wait();
   grid_release();
   if ((int)blockIdx.x < ex) {
-    const int e = blockIdx.x * 8 + warp, t0 = blockIdx.y * TG;
-    if (e >= a.E) return;
-    const uint4* wr = reinterpret_cast<const uint4*>(a.router + (long long)e * a.d);
+    const int t0 = blockIdx.y * TG;
     float acc[TG];
 #pragma unroll
     for (int t = 0; t < TG; ++t) acc[t] = 0.f;
-#pragma unroll(TG == 1 ? 8 : 2)
-    for (int c = lane; c < chunks; c += 32) {
-      const uint4 v = __ldg(wr + c);
+#pragma unroll(TG == 1 ? 4 : TG == 4 ? 3 : 2)
+    for (int c = c0; c < chunks; c += 128) {
+      const uint4 v = wr[c];
       const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int t = 0; t < TG; ++t) {
@@ -188,12 +192,17 @@ __global__ void __launch_bounds__(256) k_moe_route(MoeFp8Args a, MoeWs w) {
       }
     }
 #pragma unroll
-    for (int t = 0; t < TG; ++t) {
+    for (int o = 16; o; o >>= 1)
 #pragma unroll
-      for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(MS_FULL, acc[t], o);
-      if (lane == 0 && t0 + t < a.T)
-        w.logits[(t0 + t) * a.E + e] = acc[t] + (a.router_bias ? a.router_bias[e] : 0.f);
-    }
+      for (int t = 0; t < TG; ++t) acc[t] += __shfl_xor_sync(MS_FULL, acc[t], o);
+    if (lane == 0)
+#pragma unroll
+      for (int t = 0; t < TG; ++t) part[warp][t] = acc[t];
+    __syncthreads();
+    const int q = threadIdx.x / TG, t = threadIdx.x % TG, eo = blockIdx.x * 2 + q;
+    if (q < 2 && eo < a.E && t0 + t < a.T)
+      w.logits[(t0 + t) * a.E + eo] = ((part[4 * q][t] + part[4 * q + 1][t]) + (part[4 * q + 2][t] + part[4 * q + 3][t])) +
+                                      (a.router_bias ? a.router_bias[eo] : 0.f);
     return;
   }
   const int q = blockIdx.x - ex, nq = gridDim.x - ex;          // q-th of the quantising CTAs of this row
@@ -1132,7 +1141,7 @@ static cudaError_t launch_route(const MoeFp8Args& a, const MoeWs& w, cudaStream_
   const int rows = (a.T + TG - 1) / TG;
   // a quantising CTA per 16 groups of its share of the tokens, or per 16 KB to clear
   const int clear = TG == 1 ? (int)std::min<long long>(64, (w.words + 2047) / 2048) : 1;
-  cfg.gridDim = dim3((a.E + 7) / 8 + std::max(clear, (TG * blocks128(a.d) + 15) / 16), rows);
+  cfg.gridDim = dim3((a.E + 1) / 2 + std::max(clear, (TG * blocks128(a.d) + 15) / 16), rows);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
