@@ -193,7 +193,9 @@ def quantize_fp8(x, stream=None):
 def status(device=None, stream=None):
     """Raise if a bounded wait inside an fp8 kernel on `device` ran out since
     the last call (its output is not valid). Waits for the stream."""
-    dev = torch.cuda.current_device() if device is None else torch.device(device).index
+    dev = None if device is None else torch.device(device).index
+    if dev is None:
+        dev = torch.cuda.current_device()
     st = ctypes.c_int()
     _lib.check(_lib.load().ms_fp8_status(dev, ctypes.byref(st), ctypes.c_void_p(_stream(dev, stream))))
 
