@@ -219,24 +219,31 @@ __global__ void __launch_bounds__(FEW_THREADS)
 // before the last of them. That takes 232 registers a thread, given by the
 // warps that need none. Two products of 256 x 256 fill TMEM (four of 256 x 128
 // were slower, 266 against 260 us for 16384 x 5120 x 2880: twice the barriers).
+// A block then takes 0.48 us however few the tiles are, most of it the trip
+// between the CTAs of a pair and back. So a single CTA (PAIR false) computes
+// 128 x 128 outputs, with four buffers and barriers of its own, where its
+// tiles are few (0.39 us); it loads twice the bytes for the same tensor work.
 //
 // Warps 0-7 take products out of TMEM and write the outputs (lane quarter
-// warp % 4, column half warp / 4), warp 8 loads, warp 9 of the even CTA
+// warp % 4, column half warp / 4), warp 8 loads, warp 9 (of the even CTA)
 // issues the MMAs, 10 and 11 bring the scales into shared memory eight blocks
 // at a time (read one block ahead, their latency was the length of a step:
 // 395 us for 16384 x 5120 x 2880). The outputs go through a
-// swizzled 4 KB tile, two per warp, and a tensor store, so that whole lines are
+// swizzled 4 KB tile of the warp and a tensor store, so that whole lines are
 // written; outputs that a tensor map cannot describe are stored one by one.
-constexpr int PAIR_THREADS = 384, PAIR_STAGES = 4, PAIR_BUFS = 2;
-constexpr int PAIR_STAGE = 2 * FP8_W_TILE;
-constexpr int PAIR_OFF_OUT = PAIR_STAGES * PAIR_STAGE;
-constexpr int PAIR_CHUNK = 8;                 // blocks whose scales are staged together
-constexpr int PAIR_OFF_S = PAIR_OFF_OUT + 8 * 8192;               // [2][CHUNK][128] of x
-constexpr int PAIR_OFF_SW = PAIR_OFF_S + 2 * PAIR_CHUNK * 512;    // [2][CHUNK][2] of w
-constexpr int PAIR_OFF_B = PAIR_OFF_SW + 2 * PAIR_CHUNK * 8;      // [4][256] bias of a tile
-constexpr int PAIR_OFF_BAR = PAIR_OFF_B + 4 * 1024;
-constexpr int PAIR_SMEM = PAIR_OFF_BAR + 256 + 1024;
-static_assert(PAIR_SMEM <= 232448 && PAIR_SMEM > 232448 - 77824, "alone on its SM");
+constexpr int ROWS_THREADS = 384, ROWS_STAGE = 2 * FP8_W_TILE;
+constexpr int ROWS_CHUNK = 8;                 // blocks whose scales are staged together
+template <bool PAIR> struct Rows {
+  static constexpr int STAGES = PAIR ? 4 : 5, BUFS = PAIR ? 2 : 4;
+  static constexpr int OUTS = PAIR ? 2 : 1;                          // output tiles per warp
+  static constexpr int OFF_OUT = STAGES * ROWS_STAGE;
+  static constexpr int OFF_S = OFF_OUT + 8 * OUTS * 4096;            // [2][CHUNK][128] of x
+  static constexpr int OFF_SW = OFF_S + 2 * ROWS_CHUNK * 512;        // [2][CHUNK][2] of w
+  static constexpr int OFF_B = OFF_SW + 2 * ROWS_CHUNK * 8;          // [4][256] bias of a tile
+  static constexpr int OFF_BAR = OFF_B + 4 * 1024;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static_assert(SMEM <= 232448 && SMEM > 232448 - 77824, "alone on its SM");
+};
 
 template <int OUT>
 __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
@@ -248,30 +255,33 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int OUT>
-__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
-    k_linear_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+template <int OUT, bool PAIR>
+__global__ void __launch_bounds__(ROWS_THREADS, 1)
+    k_linear_rows(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                   const __grid_constant__ CUtensorMap tmY, int y_map, LinearArgs a) {
+  constexpr int CTAS = PAIR ? 2 : 1, TM = 128 * CTAS, TN = 128 * CTAS, COLS = TN / 2;
+  using C = Rows<PAIR>;
+  constexpr int BUFS = C::BUFS, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_OFF_BAR);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* full = bars;                     // [STAGES] both CTAs' tiles landed (even CTA's)
-  uint64_t* empty = full + PAIR_STAGES;      // [STAGES] MMAs have read them
-  uint64_t* d_full = empty + PAIR_STAGES;    // [BUFS] a product complete
-  uint64_t* d_empty = d_full + PAIR_BUFS;    // [BUFS] taken out by both CTAs (even CTA's)
-  uint64_t* s_full = d_empty + PAIR_BUFS;    // [2] a chunk's scales staged
+  uint64_t* empty = full + STAGES;      // [STAGES] MMAs have read them
+  uint64_t* d_full = empty + STAGES;    // [BUFS] a product complete
+  uint64_t* d_empty = d_full + BUFS;    // [BUFS] taken out by both CTAs (even CTA's)
+  uint64_t* s_full = d_empty + BUFS;    // [2] a chunk's scales staged
   uint64_t* s_empty = s_full + 2;            // [2] used
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(s_empty + 2);
-  float* s_x = reinterpret_cast<float*>(smem + PAIR_OFF_S);
-  float* s_w = reinterpret_cast<float*>(smem + PAIR_OFF_SW);
-  float* s_b = reinterpret_cast<float*>(smem + PAIR_OFF_B);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
-  const int kb = (a.K + 127) / 128, nt = (a.N + 255) / 256;
-  const int tiles = nt * ((a.M + 255) / 256), step = gridDim.x / 2;
+  float* s_x = reinterpret_cast<float*>(smem + C::OFF_S);
+  float* s_w = reinterpret_cast<float*>(smem + C::OFF_SW);
+  float* s_b = reinterpret_cast<float*>(smem + C::OFF_B);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? blockIdx.x & 1 : 0;
+  const int kb = (a.K + 127) / 128, nt = (a.N + TN - 1) / TN;
+  const int tiles = nt * ((a.M + TM - 1) / TM), first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < PAIR_STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < PAIR_BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 16);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < BUFS; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 8 * CTAS);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 2), mbar_init(&s_empty[i], 8);
     fence_barrier_init();
   }
@@ -279,58 +289,75 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
     tma_map_prefetch(&tmW);
     tma_map_prefetch(&tmX);
   }
-  if (warp == 9) tmem_get2(tmem_at, 512);
+  if (warp == 9) {
+    if (PAIR) tmem_get2(tmem_at, 512);
+    else tmem_get(tmem_at, 512);
+  }
   tc_before();
-  cluster_sync();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   tc_after();
   const uint32_t tmem = *tmem_at;
   grid_wait();
   grid_release();
 
   if (warp >= 8) {
-    regs_down<40>();
+    if (PAIR) regs_down<40>();
     if (warp == 8) {
-      const uint32_t full_even = cluster_map(full, 0);
+      const uint32_t full_even = PAIR ? cluster_map(full, 0) : 0;
       bool ok = true;
       int i = 0;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += step) {
-        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256 + rank * 128;
+      for (int t = first; t < tiles && ok; t += step) {
+        const int m0 = t / nt * TM + rank * 128, n0 = t % nt * TN + rank * 128;
         for (int b = 0; b < kb; ++b, ++i) {
-          const int s = i % PAIR_STAGES;
-          if (i >= PAIR_STAGES && !mbar_wait_step(&empty[s], ((i / PAIR_STAGES) - 1) & 1, &g_linear_status)) {
-            for (int j = i - PAIR_STAGES; j < i && rank == 0; ++j)
-              mbar_wait(&full[j % PAIR_STAGES], (j / PAIR_STAGES) & 1, &g_linear_status);
+          const int s = i % STAGES;
+          if (i >= STAGES && !mbar_wait_step(&empty[s], ((i / STAGES) - 1) & 1, &g_linear_status)) {
+            for (int j = i - STAGES; j < i && rank == 0; ++j)
+              mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &g_linear_status);
             ok = false;
             break;
           }
           if (elect_one()) {
-            if (rank == 0) mbar_expect_tx(&full[s], 2 * PAIR_STAGE);
-            uint8_t* at = smem + s * PAIR_STAGE;
-            tma_tile_pair(at, &tmX, b * 128, m0, full_even + 8 * s);
-            tma_tile_pair(at + FP8_W_TILE, &tmW, b * 128, n0, full_even + 8 * s);
+            if (rank == 0) mbar_expect_tx(&full[s], CTAS * ROWS_STAGE);
+            uint8_t* at = smem + s * ROWS_STAGE;
+            if (PAIR) {
+              tma_tile_pair(at, &tmX, b * 128, m0, full_even + 8 * s);
+              tma_tile_pair(at + FP8_W_TILE, &tmW, b * 128, n0, full_even + 8 * s);
+            } else {
+              tma_tile_2d(at, &tmX, b * 128, m0, &full[s]);
+              tma_tile_2d(at + FP8_W_TILE, &tmW, b * 128, n0, &full[s]);
+            }
           }
           __syncwarp();
         }
       }
     } else if (warp == 9 && rank == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(256, 256);
+      constexpr uint32_t idesc = idesc_e4m3(TM, TN);
       bool ok = true;
       int i = 0;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += step)
+      for (int t = first; t < tiles && ok; t += step)
         for (int b = 0; b < kb; ++b, ++i) {
-          const int s = i % PAIR_STAGES, u = i & 1;
-          if (!mbar_wait_step(&full[s], (i / PAIR_STAGES) & 1, &g_linear_status) ||
-              (i >= 2 && !mbar_wait_step(&d_empty[u], ((i >> 1) - 1) & 1, &g_linear_status))) {
+          const int s = i % STAGES, u = i % BUFS;
+          if (!mbar_wait_step(&full[s], (i / STAGES) & 1, &g_linear_status) ||
+              (i >= BUFS && !mbar_wait_step(&d_empty[u], ((i / BUFS) - 1) & 1, &g_linear_status))) {
             ok = false;
             break;
           }
           tc_after();
           if (elect_one()) {
-            const uint64_t ad = k128_desc(smem + s * PAIR_STAGE), bd = k128_desc(smem + s * PAIR_STAGE + FP8_W_TILE);
+            const uint64_t ad = k128_desc(smem + s * ROWS_STAGE), bd = k128_desc(smem + s * ROWS_STAGE + FP8_W_TILE);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma_e4m3_pair(tmem + u * 256, ad + 2 * j, bd + 2 * j, idesc, j != 0);
-            mma_done_pair(&d_full[u]);
-            mma_done_pair(&empty[s]);
+            for (int j = 0; j < 4; ++j) {
+              if (PAIR) mma_e4m3_pair(tmem + u * TN, ad + 2 * j, bd + 2 * j, idesc, j != 0);
+              else mma_e4m3(tmem + u * TN, ad + 2 * j, bd + 2 * j, idesc, j != 0);
+            }
+            if (PAIR) {
+              mma_done_pair(&d_full[u]);
+              mma_done_pair(&empty[s]);
+            } else {
+              mma_done(&d_full[u]);
+              mma_done(&empty[s]);
+            }
           }
           __syncwarp();
         }
@@ -338,106 +365,103 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
       const int r = (warp - 10) * 32 + lane;
       bool ok = true;
       int q = 0, tb = 0;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += step, tb = (tb + 1) & 3) {
-        const int m0 = t / nt * 256 + rank * 128, n0 = t % nt * 256;
+      for (int t = first; t < tiles && ok; t += step, tb = (tb + 1) & 3) {
+        const int m0 = t / nt * TM + rank * 128, n0 = t % nt * TN;
         const float* x0 = a.xs + (long long)min(m0 + r, a.M - 1) * a.xs_stride;
         const float* x1 = a.xs + (long long)min(m0 + r + 64, a.M - 1) * a.xs_stride;
         // the right half's scales, where the tile has one
-        const float* w = a.ws + (long long)(n0 / 128 + ((lane & 1) && n0 + 128 < a.N ? 1 : 0)) * kb;
-        for (int b0 = 0; b0 < kb; b0 += PAIR_CHUNK, ++q) {
-          float v0[PAIR_CHUNK], v1[PAIR_CHUNK];
+        const float* w = a.ws + (long long)(n0 / 128 + (PAIR && (lane & 1) && n0 + 128 < a.N ? 1 : 0)) * kb;
+        for (int b0 = 0; b0 < kb; b0 += ROWS_CHUNK, ++q) {
+          float v0[ROWS_CHUNK], v1[ROWS_CHUNK];
 #pragma unroll
-          for (int j = 0; j < PAIR_CHUNK; ++j) {
+          for (int j = 0; j < ROWS_CHUNK; ++j) {
             const int b = min(b0 + j, kb - 1);
             v0[j] = __ldg(x0 + b), v1[j] = __ldg(x1 + b);
           }
-          const float vw = __ldg(w + min(b0 + ((lane >> 1) & (PAIR_CHUNK - 1)), kb - 1));
+          const float vw = __ldg(w + min(b0 + ((lane >> 1) & (ROWS_CHUNK - 1)), kb - 1));
           const int u = q & 1;
           if (q >= 2 && !mbar_wait_step(&s_empty[u], ((q >> 1) - 1) & 1, &g_linear_status)) {
             ok = false;
             break;
           }
 #pragma unroll
-          for (int j = 0; j < PAIR_CHUNK; ++j) {
-            s_x[(u * PAIR_CHUNK + j) * 128 + r] = v0[j];
-            s_x[(u * PAIR_CHUNK + j) * 128 + r + 64] = v1[j];
+          for (int j = 0; j < ROWS_CHUNK; ++j) {
+            s_x[(u * ROWS_CHUNK + j) * 128 + r] = v0[j];
+            s_x[(u * ROWS_CHUNK + j) * 128 + r + 64] = v1[j];
           }
-          if (warp == 10 && lane < 2 * PAIR_CHUNK) s_w[u * 2 * PAIR_CHUNK + lane] = vw;
+          if (warp == 10 && lane < 2 * ROWS_CHUNK) s_w[u * 2 * ROWS_CHUNK + lane] = vw;
           // a tile's bias lies there until its outputs are written: by then this
           // warp is at most three tiles further
           if (b0 == 0 && a.bias)
-            for (int n = r; n < 256; n += 64) s_b[tb * 256 + n] = n0 + n < a.N ? __ldg(a.bias + n0 + n) : 0.f;
+            for (int n = r; n < TN; n += 64) s_b[tb * 256 + n] = n0 + n < a.N ? __ldg(a.bias + n0 + n) : 0.f;
           __syncwarp();
           if (lane == 0) mbar_arrive1(&s_full[u]);
         }
       }
     }
   } else {
-    regs_up<232>();
-    const uint32_t d_empty_even = cluster_map(d_empty, 0);
+    if (PAIR) regs_up<232>();
+    const uint32_t d_empty_even = PAIR ? cluster_map(d_empty, 0) : 0;
     const int quarter = warp & 3, half = warp >> 2;
-    uint8_t* outs = smem + PAIR_OFF_OUT + warp * 8192;
+    uint8_t* outs = smem + C::OFF_OUT + warp * (C::OUTS * 4096);
     int i = 0, q = 0, tb = 0, ob = 0;
     bool ok = true;
-    const uint32_t d0 = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
-    for (int t = blockIdx.x / 2; t < tiles; t += step, tb = (tb + 1) & 3) {
-      const int m = t / nt * 256 + rank * 128 + quarter * 32 + lane, n0 = t % nt * 256 + half * 128;
-      float acc[128];
+    const uint32_t d0 = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+    for (int t = first; t < tiles; t += step, tb = (tb + 1) & 3) {
+      const int m = t / nt * TM + rank * 128 + quarter * 32 + lane, n0 = t % nt * TN + half * COLS;
+      float acc[COLS];
 #pragma unroll
-      for (int n = 0; n < 128; ++n) acc[n] = 0.f;
-      uint32_t v0[32], v1[32];
-      ok = mbar_wait_step(&d_full[i & 1], (i >> 1) & 1, &g_linear_status);
+      for (int n = 0; n < COLS; ++n) acc[n] = 0.f;
+      uint32_t v[2][32];
+      ok = mbar_wait_step(&d_full[i % BUFS], (i / BUFS) & 1, &g_linear_status);
       if (!ok) break;
       tc_after();
-      tmem_load32(d0 + (i & 1) * 256, v0);
+      tmem_load32(d0 + i % BUFS * TN, v[0]);
       for (int b = 0; b < kb; ++b, ++i) {
-        const int sb = b % PAIR_CHUNK, su = q & 1;
-        const bool chunk_end = sb == PAIR_CHUNK - 1 || b == kb - 1;
+        const int sb = b % ROWS_CHUNK, su = q & 1;
+        const bool chunk_end = sb == ROWS_CHUNK - 1 || b == kb - 1;
         if (sb == 0) ok = mbar_wait_step(&s_full[su], (q >> 1) & 1, &g_linear_status);
         if (!ok) break;
         const uint64_t ff =
-            twice(s_x[(su * PAIR_CHUNK + sb) * 128 + quarter * 32 + lane] * s_w[(su * PAIR_CHUNK + sb) * 2 + half]);
-        const uint32_t d = d0 + (i & 1) * 256;
-        tmem_wait32(v0);
-        tmem_load32(d + 32, v1);
+            twice(s_x[(su * ROWS_CHUNK + sb) * 128 + quarter * 32 + lane] * s_w[(su * ROWS_CHUNK + sb) * 2 + half]);
+        const uint32_t d = d0 + i % BUFS * TN;
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) fma2(acc[j], acc[j + 1], v0[j], v0[j + 1], ff);
-        tmem_wait32(v1);
-        tmem_load32(d + 64, v0);
+        for (int c = 0; c < COLS; c += 32) {
+          uint32_t *now = v[c / 32 & 1], *next = v[c / 32 & 1 ^ 1];
+          tmem_wait32(now);
+          if (c + 32 < COLS) {
+            tmem_load32(d + c + 32, next);
+          } else {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(d_empty_even + 8 * (i % BUFS));
+              else mbar_arrive1(&d_empty[i % BUFS]);
+              if (chunk_end) mbar_arrive1(&s_empty[su]);
+            }
+            q += chunk_end;
+            if (b + 1 < kb) {
+              ok = mbar_wait_step(&d_full[(i + 1) % BUFS], ((i + 1) / BUFS) & 1, &g_linear_status);
+              tc_after();
+              tmem_load32(d0 + (i + 1) % BUFS * TN, next);
+            }
+          }
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) fma2(acc[32 + j], acc[33 + j], v1[j], v1[j + 1], ff);
-        tmem_wait32(v0);
-        tmem_load32(d + 96, v1);
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) fma2(acc[64 + j], acc[65 + j], v0[j], v0[j + 1], ff);
-        tmem_wait32(v1);
-        tc_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_cluster(d_empty_even + 8 * (i & 1));
-          if (chunk_end) mbar_arrive1(&s_empty[su]);
+          for (int j = 0; j < 32; j += 2) fma2(acc[c + j], acc[c + j + 1], now[j], now[j + 1], ff);
         }
-        q += chunk_end;
-        if (b + 1 < kb) {
-          ok = mbar_wait_step(&d_full[(i + 1) & 1], ((i + 1) >> 1) & 1, &g_linear_status);
-          tc_after();
-          tmem_load32(d0 + ((i + 1) & 1) * 256, v0);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) fma2(acc[96 + j], acc[97 + j], v1[j], v1[j + 1], ff);
       }
       if (!ok) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < COLS / 64; ++h) {
         const int c0 = n0 + 64 * h;
         if (c0 >= a.N) break;
-        float* v = acc + 64 * h;
+        float* o64 = acc + 64 * h;
         if (a.bias) {
-          const float4* b4 = reinterpret_cast<const float4*>(s_b + tb * 256 + half * 128 + 64 * h);
+          const float4* b4 = reinterpret_cast<const float4*>(s_b + tb * 256 + half * COLS + 64 * h);
 #pragma unroll
           for (int n = 0; n < 16; ++n) {
             const float4 bias = b4[n];
-            v[4 * n] += bias.x, v[4 * n + 1] += bias.y, v[4 * n + 2] += bias.z, v[4 * n + 3] += bias.w;
+            o64[4 * n] += bias.x, o64[4 * n + 1] += bias.y, o64[4 * n + 2] += bias.z, o64[4 * n + 3] += bias.w;
           }
         }
         if (y_map) {
@@ -448,16 +472,17 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               if (OUT == DT_F32) {
-                o[j] = make_uint4(__float_as_uint(v[c + 4 * j]), __float_as_uint(v[c + 4 * j + 1]),
-                                  __float_as_uint(v[c + 4 * j + 2]), __float_as_uint(v[c + 4 * j + 3]));
+                o[j] = make_uint4(__float_as_uint(o64[c + 4 * j]), __float_as_uint(o64[c + 4 * j + 1]),
+                                  __float_as_uint(o64[c + 4 * j + 2]), __float_as_uint(o64[c + 4 * j + 3]));
               } else {
-                o[j] = make_uint4(pack_out<OUT>(v[8 * j], v[8 * j + 1]), pack_out<OUT>(v[8 * j + 2], v[8 * j + 3]),
-                                  pack_out<OUT>(v[8 * j + 4], v[8 * j + 5]), pack_out<OUT>(v[8 * j + 6], v[8 * j + 7]));
+                o[j] = make_uint4(pack_out<OUT>(o64[8 * j], o64[8 * j + 1]), pack_out<OUT>(o64[8 * j + 2], o64[8 * j + 3]),
+                                  pack_out<OUT>(o64[8 * j + 4], o64[8 * j + 5]), pack_out<OUT>(o64[8 * j + 6], o64[8 * j + 7]));
               }
             }
-            tma_store_read_wait();                   // lane 0 sent the tile before the last
+            tma_store_read_wait<C::OUTS - 1>();      // lane 0 sent the tile that lay here
             __syncwarp();
-            uint8_t* out = outs + (ob ^= 4096);
+            uint8_t* out = outs + ob;
+            if (C::OUTS == 2) ob ^= 4096;
 #pragma unroll
             for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(out + lane * 128 + ((j ^ (lane & 7)) << 4)) = o[j];
             fence_async_shared();
@@ -467,15 +492,19 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
         } else if (m < a.M) {
 #pragma unroll
           for (int n = 0; n < 64; ++n)
-            if (c0 + n < a.N) store_out<OUT>(a.y, m * a.y_stride + c0 + n, v[n]);
+            if (c0 + n < a.N) store_out<OUT>(a.y, m * a.y_stride + c0 + n, o64[n]);
         }
       }
     }
     if (lane == 0) tma_store_wait();
   }
   tc_before();
-  cluster_sync();                            // the even CTA's barriers serve both to the end
-  if (warp == 9) tmem_free2(tmem, 512);
+  if (PAIR) cluster_sync();                  // the even CTA's barriers serve both to the end
+  else __syncthreads();
+  if (warp == 9) {
+    if (PAIR) tmem_free2(tmem, 512);
+    else tmem_free(tmem, 512);
+  }
 }
 
 // ------------------------------------------------------------------ launches
@@ -557,27 +586,30 @@ static bool encode_out_map(CUtensorMap* m, const LinearArgs& a) {
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int OUT>
-static cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t s) {
-  const long long tiles = (long long)((a.N + 255) / 256) * ((a.M + 255) / 256);
+template <int OUT, bool PAIR>
+static cudaError_t launch_rows(const LinearArgs& a, int sms, cudaStream_t s) {
+  constexpr int CTAS = PAIR ? 2 : 1, T = 128 * CTAS;
+  const long long tiles = (long long)((a.N + T - 1) / T) * ((a.M + T - 1) / T);
   CUtensorMap tw, tx, ty{};
   if (encode_fp8_map(&tw, a.w, a.K, a.N, a.w_stride, 128, 0, 0) ||
       encode_fp8_map(&tx, a.x, a.K, a.M, a.x_stride, 128, 0, 0))
     return cudaErrorInvalidValue;
   const int y_map = encode_out_map<OUT>(&ty, a);
-  auto kern = k_linear_pair<OUT>;
-  cudaError_t e = allow_shared<k_linear_pair<OUT>>(PAIR_SMEM);
+  auto kern = k_linear_rows<OUT, PAIR>;
+  cudaError_t e = allow_shared<k_linear_rows<OUT, PAIR>>(Rows<PAIR>::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, sms / 2) * 2);
-  cfg.blockDim = dim3(PAIR_THREADS);
-  cfg.dynamicSmemBytes = PAIR_SMEM;
+  cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, sms / CTAS) * CTAS);
+  cfg.blockDim = dim3(ROWS_THREADS);
+  cfg.dynamicSmemBytes = Rows<PAIR>::SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, tw, tx, ty, y_map, a);
 }
 
@@ -586,14 +618,16 @@ static cudaError_t launch_out(const LinearArgs& a, int sms, cudaStream_t s) {
   if (a.M <= 16) return launch_few<16, OUT>(a, sms, s);
   if (a.M <= 32) return launch_few<32, OUT>(a, sms, s);
   if (a.M <= 64) return launch_few<64, OUT>(a, sms, s);
-  // Beyond 64 rows the weight is read more than once by the first kernel, and
-  // the second needs tiles for its pairs: the first is ahead while its
-  // 128 x 64 tiles fit the GPU at once (us, first / second: M 128, N 5120, K
-  // 2048 11.9 / 12.0; M 384, N 2880, K 4096 18.2 / 19.7; M 512, N 1024, K 4096
-  // 13.6 / 19.6), behind once they do not (M 256, N 5120, K 2048 15.2 / 12.1;
-  // M 512, N 2880, K 4096 25.7 / 19.8).
-  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) <= sms) return launch_few<64, OUT>(a, sms, s);
-  return launch_pair<OUT>(a, sms, s);
+  // Beyond 64 rows: the first kernel while its 128 x 64 tiles leave room to
+  // cut a long K between CTAs, then single CTAs while their 128 x 128 tiles fit
+  // the GPU at once, then pairs (us, in this order: M 128, N 2880, K 4096 11.7,
+  // 16.2, 19.6; M 512, N 1024, K 4096 11.6, 16.2, 19.8; M 333, N 5120, K 2880
+  // 20.1, 13.3, 16.0; M 128, N 5120, K 2048 12.0, 10.0, 12.1; M 512, N 5120, K
+  // 2880 35.4, 22.3, 16.3; K 512 a draw of the first two).
+  const long long rows = (a.N + 127) / 128;
+  if (a.K > 1024 && 2 * rows * ((a.M + 63) / 64) <= sms) return launch_few<64, OUT>(a, sms, s);
+  if (rows * ((a.M + 127) / 128) <= sms) return launch_rows<OUT, false>(a, sms, s);
+  return launch_rows<OUT, true>(a, sms, s);
 }
 
 cudaError_t launch_linear_fp8(const LinearArgs& a, int out_dtype, int sms, cudaStream_t s) {
