@@ -177,7 +177,8 @@ def check_linear(y, xq, xs, wq, ws, bias, dt):
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8, 16), (1, 5120, 2048), (2, 130, 127), (3, 64, 128), (16, 2880, 4096),
                                    (17, 129, 129), (31, 500, 320), (33, 513, 1000), (64, 768, 2048), (65, 256, 640),
                                    (100, 2880, 2880), (128, 128, 128), (129, 385, 272), (200, 1024, 96), (256, 256, 256),
-                                   (300, 640, 2880), (513, 5120, 400), (1000, 333, 2049)])
+                                   (300, 640, 2880), (513, 5120, 400), (1000, 333, 2049),
+                                   (333, 5120, 2880), (70, 8200, 1030), (1500, 3000, 1160), (64, 20000, 144)])
 def test_linear(M, N, K, dt, lib, cuda):
     from moe_stream_b200 import fp8
     g = _gen(M * 7 + N * 3 + K)
@@ -518,6 +519,24 @@ def test_chain_captured_replayed_and_on_other_streams(lib, cuda):
     qx, sx = O.quantize(t)
     assert torch.equal(q2.double(), qx) and torch.equal(s2.double(), sx)
     assert torch.equal(y, c[4][0](ins[0][0], residual=h2))
+
+
+def test_layer_on_streams_at_once(lib, cuda):
+    """Full layers of one and of many tokens on four streams: whichever SMs a
+    call gets, its outputs are those of the call alone."""
+    g = _gen(34)
+    layer = make_moe(g, "qwen3", 2048, 768, 64, 8)[0]
+    xs = [_tokens(g, n, 2048) for n in (1, 1, 20, 64)]
+    want = [layer(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(layer(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_chain_leaves_its_inputs_and_neighbours_alone(lib, cuda):
