@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(TPR ? TPR : 512) k_norm_fp8(NormArgs a) {
         ss += squares(v);
       }
       if (PIPE && t + (int)gridDim.x < a.T) fetch(t + gridDim.x);    // h may be x or res: another row
-      if (a.res) {
+      if (a.h) {
         E* o = static_cast<E*>(a.h) + t * a.h_stride;
 #pragma unroll
         for (int i = 0; i < NC; ++i)

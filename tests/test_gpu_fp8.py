@@ -152,6 +152,23 @@ def test_norm_strides_shapes_and_in_place(lib, cuda):
     assert e[0].shape == (0, 250) and e[1].shape == (0, 2) and e[2].shape == (0, 250)
 
 
+@pytest.mark.parametrize("T,d", [(3, 256), (2, 250), (700, 768)])
+def test_norm_writes_h_without_a_residual(T, d, lib, cuda):
+    """The C entry takes h without a residual: h is x then, in h's own stride."""
+    from moe_stream_b200 import fp8
+    g = _gen(d)
+    x, w = _rows(g, T, d, "bf16"), _rows(g, 1, d, "bf16")[0]
+    want = fp8.rms_norm_fp8(x, w)
+    wide = torch.full((T, d + 22), 7.0, dtype=torch.bfloat16, device="cuda")
+    q, s = torch.empty_like(want[0]), torch.empty_like(want[1])
+    dev = x.get_device()
+    args = fp8._NORM.pack(x.data_ptr(), 0, w.data_ptr(), wide.data_ptr(), 0, q.data_ptr(), s.data_ptr(),
+                          d, 0, d + 22, 0, q.stride(0), 1e-6, T, d, 0, dev)
+    assert lib.ms_rms_norm_fp8(args, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(wide[:, :d], x) and (wide[:, d:] == 7.0).all()
+    assert torch.equal(q.view(torch.uint8), want[0].contiguous().view(torch.uint8)) and torch.equal(s, want[1])
+
+
 # ------------------------------------------------------------------- linear
 def _codes(g, M, K, pad_with=0x7F):
     """Codes [M, K] in rows padded to 16 bytes with NaN codes, and scales that
