@@ -169,6 +169,21 @@ def test_norm_writes_h_without_a_residual(T, d, lib, cuda):
     assert torch.equal(q.view(torch.uint8), want[0].contiguous().view(torch.uint8)) and torch.equal(s, want[1])
 
 
+def test_norm_offsets_past_32_bits(lib, cuda):
+    """More than 2^31 features: rows do not depend on their neighbours."""
+    from moe_stream_b200 import fp8
+    g = _gen(21)
+    T, d = (1 << 20) + 37, 2048
+    x = torch.randn(T, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = _rows(g, 1, d, "bf16")[0]
+    for run in (lambda v: fp8.quantize_fp8(v), lambda v: fp8.rms_norm_fp8(v, w, residual=v)):
+        got = run(x)
+        for at in (0, T // 2, T - 64):
+            for a, b in zip(got, run(x[at:at + 64])):
+                assert torch.equal(a[at:at + 64].view(torch.uint8), b.view(torch.uint8))
+        del got
+
+
 # ------------------------------------------------------------------- linear
 def _codes(g, M, K, pad_with=0x7F):
     """Codes [M, K] in rows padded to 16 bytes with NaN codes, and scales that
@@ -223,6 +238,30 @@ def test_linear_large(lib, cuda):
         m1 = min(M, m0 + 1024)
         check_linear(y[m0:m1], xq[m0:m1], xs[m0:m1], wq, ws, None, "bf16")
     assert torch.equal(y, lin(xq, xs))
+
+
+@pytest.mark.parametrize("M,N,K", [(524400, 4104, 128), (524400, 4099, 128), (131300, 136, 16384), (3, 131200, 16400),
+                                   (150, 131200, 16400)])
+def test_linear_offsets_past_32_bits(M, N, K, lib, cuda):
+    """More than 2^31 outputs, by tensor stores and one by one, activations
+    and weights: parts at both ends."""
+    from moe_stream_b200 import fp8
+    g = _gen(M + N)
+
+    def codes(n):
+        c = torch.randint(0, 0x60, (n, K), generator=g, device="cuda", dtype=torch.uint8)
+        c[:, ::3] |= 0x80
+        return c.view(torch.float8_e4m3fn)
+
+    kb = -(-K // 128)
+    xq, wq = codes(M), codes(N)
+    xs = torch.rand(M, kb, generator=g, device="cuda") + 0.5
+    ws = (torch.rand(-(-N // 128), kb, generator=g, device="cuda") + 0.5) * 2.0 ** -12
+    y = fp8.Fp8Linear(wq, ws)(xq, xs)
+    for m in {0, max(0, M - 130)}:
+        for n in {0, (N - 1) // 128 * 128 - 128}:
+            check_linear(y[m:m + 130, n:n + 256], xq[m:m + 130], xs[m:m + 130], wq[n:n + 256],
+                         ws[n // 128:n // 128 + 2], None, "bf16")
 
 
 @pytest.mark.parametrize("M", [5, 40, 300])
