@@ -392,6 +392,26 @@ def test_moe(model, T, d, f, E, k, lib, cuda):
     assert torch.equal(y, layer(x)), "two calls on the same inputs differ"
 
 
+@pytest.mark.parametrize("T", [1, 6, 40])
+def test_moe_offsets_past_32_bits(T, lib, cuda):
+    """More than 2^31 codes a matrix; the last experts are the ones chosen."""
+    from moe_stream_b200 import fp8
+    g = _gen(28)
+    d, f, E, k = 2064, 4096, 256, 4
+    router = (torch.randn(E, d, generator=g, device="cuda") * 0.05).to(torch.bfloat16)
+    rb = torch.zeros(E, device="cuda")
+    rb[E - 8:] = 40.0
+    parts = []
+    for n, m in ((f, d), (f, d), (d, f)):
+        c = torch.randint(0, 0x60, (E, n, m), generator=g, device="cuda", dtype=torch.uint8)
+        c[:, :, ::3] |= 0x80
+        s = (torch.rand(E, -(-n // 128), -(-m // 128), generator=g, device="cuda") + 0.5) * 2.0 ** -10
+        parts.append((c.view(torch.float8_e4m3fn), s, None))
+    x = _tokens(g, T, d)
+    y = fp8.Fp8MoELayer("qwen3", router, *parts, top_k=k, router_bias=rb)(x)
+    check_moe(y, x, router, rb, parts, k, "qwen3")
+
+
 def test_moe_without_renormalisation_and_with_biases(lib, cuda):
     g = _gen(21)
     for bias in (False, True):
