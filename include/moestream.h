@@ -485,6 +485,14 @@ int ms_moe_fp8_layer(const ms_fp8_moe* args, void* stream);
  * Waits for `stream`; not for use in a capture. */
 int ms_fp8_status(int device, int* status, void* stream);
 
+/* Failure-detection self-test, no reference counterpart: ms_moe_fp8_layer's
+ * arguments with T above 12, of which the experts' kernel alone is enqueued,
+ * over a workspace in which no token is ever routed. Every CTA's wait for the
+ * routing gives up after a second, the kernel ends without reading an expert
+ * or writing y, and ms_fp8_status reports MS_E_TIMEOUT. Calls before and after
+ * it are not affected. */
+int ms_fp8_selftest_wait(const ms_fp8_moe* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

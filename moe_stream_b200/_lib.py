@@ -114,6 +114,7 @@ EXPORTS = {
     "ms_moe_fp8_workspace": [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)],
     "ms_moe_fp8_layer": [ctypes.c_char_p, ctypes.c_void_p],
     "ms_fp8_status": [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_void_p],
+    "ms_fp8_selftest_wait": [ctypes.c_char_p, ctypes.c_void_p],
 }
 
 _LIB = None

@@ -87,6 +87,11 @@ struct MoeFp8Args {
 };
 size_t moe_fp8_workspace(int T, int d, int f, int E, int k);
 cudaError_t launch_moe_fp8(const MoeFp8Args& a, int sms, cudaStream_t s);
+// Self-test of the layer's waits, for more than MOE_FP8_ROUTED_HERE tokens (up
+// to that many are routed by every CTA for itself, without a wait): no token
+// is ever routed. y and the experts are not touched.
+constexpr int MOE_FP8_ROUTED_HERE = 12;
+cudaError_t launch_moe_fp8_lost(const MoeFp8Args& a, int sms, cudaStream_t s);
 // Address, on the current device, of the status word of the layer's kernels.
 cudaError_t moe_fp8_status(int** at);
 

@@ -133,8 +133,10 @@ extern "C" int ms_moe_fp8_workspace(const ms_fp8_moe* p, size_t* bytes) {
   return MS_OK;
 }
 
-extern "C" int ms_moe_fp8_layer(const ms_fp8_moe* p, void* stream) {
-  const char* me = "ms_moe_fp8_layer";
+namespace {
+using MoeLaunch = cudaError_t (*)(const MoeFp8Args&, int, cudaStream_t);
+
+int moe_call(const char* me, const ms_fp8_moe* p, void* stream, MoeLaunch launch) {
   const int rc = check_moe(me, p);
   if (rc) return rc;
   if (p->T == 0) return MS_OK;
@@ -160,7 +162,21 @@ extern "C" int ms_moe_fp8_layer(const ms_fp8_moe* p, void* stream) {
   a.ws = static_cast<uint8_t*>(p->workspace);
   a.model = p->model, a.T = p->T, a.d = p->d_model, a.f = p->d_ff, a.E = p->n_experts, a.k = p->top_k;
   a.norm_topk = p->norm_topk_prob;
-  return launched(me, launch_moe_fp8(a, sm_count(p->device), static_cast<cudaStream_t>(stream)));
+  return launched(me, launch(a, sm_count(p->device), static_cast<cudaStream_t>(stream)));
+}
+}  // namespace
+
+extern "C" int ms_moe_fp8_layer(const ms_fp8_moe* p, void* stream) {
+  return moe_call("ms_moe_fp8_layer", p, stream, launch_moe_fp8);
+}
+
+extern "C" int ms_fp8_selftest_wait(const ms_fp8_moe* p, void* stream) {
+  const char* me = "ms_fp8_selftest_wait";
+  const int rc = check_moe(me, p);
+  if (rc) return rc;
+  if (p->T <= MOE_FP8_ROUTED_HERE)
+    return bad(MS_E_INVALID, "%s: T must be above %d (fewer tokens are routed without a wait)", me, MOE_FP8_ROUTED_HERE);
+  return moe_call(me, p, stream, launch_moe_fp8_lost);
 }
 
 extern "C" int ms_fp8_status(int device, int* status, void* stream) {

@@ -56,7 +56,9 @@
 
 namespace ms {
 
-// first failure of a bounded wait in this file's kernels (ms_fp8_status)
+// first failure of a bounded wait in this file's kernels (ms_fp8_status). For
+// reporting alone: what a call does after a wait that ran out goes by the word
+// in its own workspace, so it does not outlive the call or reach another.
 static __device__ int g_moe_status;
 
 namespace {
@@ -64,6 +66,8 @@ namespace {
 constexpr int MOE_FAC = 16;            // blocks of a task at most
 constexpr int MOE_SPLIT = 8;           // ranges of a tile's blocks at most
 constexpr int COMBINE_T = 4;           // tokens of a combine task, one per warp
+constexpr int MOE_THREADS = 384, MOE_ROWS = 8;    // MOE_ROWS: rows of activations passed on at a time
+static_assert(MOE_THREADS / 32 == MOE_FP8_ROUTED_HERE, "a warp per token");
 
 __host__ __device__ inline int blocks128(int n) { return (n + 127) / 128; }
 inline long long up16(long long n) { return (n + 15) / 16 * 16; }
@@ -92,6 +96,7 @@ struct MoeWs {            // workspace layout
   unsigned* next;         // next task; this and the following are zeroed by k_moe_route
   unsigned* rt_next;      // next token to route
   unsigned* routed;       // tokens routed
+  int* failed;            // ST_E_TIMEOUT once a wait of this call has run out
   unsigned* brought;      // [up tile] ranges brought
   unsigned* flag;         // [up tile] its block is quantised
   unsigned* dn_done;      // [tile of d] warps that are done with down tasks
@@ -152,9 +157,10 @@ static long long layout_ws(uint8_t* w, int T, int d, int f, int E, int k, int ct
   o->inds = reinterpret_cast<int*>(w), w += up16(4 * P);
   o->probs = reinterpret_cast<float*>(w), w += up16(4 * P);
   o->next = reinterpret_cast<unsigned*>(w), o->rt_next = o->next + 1, o->routed = o->next + 2;
-  o->brought = o->next + 3, o->flag = o->brought + tiles, o->dn_done = o->flag + tiles;
+  o->failed = reinterpret_cast<int*>(o->next + 3);
+  o->brought = o->next + 4, o->flag = o->brought + tiles, o->dn_done = o->flag + tiles;
   o->up_done = o->dn_done + blocks128(d);
-  o->counters = 4 + 2 * tiles + blocks128(d);
+  o->counters = 5 + 2 * tiles + blocks128(d);
   w += up16(4ll * o->counters);
   return w - base;
 }
@@ -241,7 +247,6 @@ __global__ void __launch_bounds__(256) k_moe_route(MoeFp8Args a, MoeWs w) {
 }
 
 // ------------------------------------------------------------------- experts
-constexpr int MOE_THREADS = 384, MOE_ROWS = 8;    // rows of activations passed on at a time
 template <int NT> struct Moe {
   static constexpr int ACT = NT <= 32 ? 4096 : NT * 128;             // activation tiles of a step
   static constexpr int STAGE = 2 * FP8_W_TILE + ACT;
@@ -304,6 +309,17 @@ __device__ __forceinline__ int choose_split(int n, int kb, int ctas, int cap, fl
   return __ffs(__ballot_sync(MS_FULL, key == least));
 }
 
+// Records that a wait of the call whose word `failed` is ran out.
+__device__ __forceinline__ void wait_ran_out(int* failed) {
+  atomicExch(failed, ST_E_TIMEOUT);
+  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
+}
+__device__ __forceinline__ bool wait_step(uint64_t* bar, unsigned phase, int* failed) {
+  if (mbar_wait_step(bar, phase, nullptr)) return true;
+  wait_ran_out(failed);
+  return false;
+}
+
 // A value and its mark in one word, written and read whole.
 __device__ __forceinline__ void put_word(unsigned long long* p, uint32_t v) {
   asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(1ull << 32 | v) : "memory");
@@ -313,10 +329,8 @@ __device__ __forceinline__ unsigned long long get_word(const unsigned long long*
   asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
-// v[q] = the value of word p[q * stride] for q < n, once all are written; a
-// second at most.
-// Four words from each of four places, as wait_words.
-__device__ __forceinline__ void wait_quads(const unsigned long long* const* p, uint32_t (*v)[4]) {
+// Four words from each of four places, once all are written; a second at most.
+__device__ __forceinline__ void wait_quads(const unsigned long long* const* p, uint32_t (*v)[4], int* failed) {
   unsigned long long t0 = 0;
   for (unsigned i = 0;; ++i) {
     unsigned have = 0;
@@ -333,13 +347,15 @@ __device__ __forceinline__ void wait_quads(const unsigned long long* const* p, u
     if ((i & 63) == 63) {
       const unsigned long long now = global_ns();
       if (!t0) t0 = now;
-      if (now - t0 > MBAR_WAIT_NS || timed_out(&g_moe_status)) break;
+      if (now - t0 > MBAR_WAIT_NS || timed_out(failed)) break;
     }
   }
-  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
+  wait_ran_out(failed);
 }
+// v[q] = the value of word p[q * stride] for q < n, as wait_quads.
 template <int N>
-__device__ __forceinline__ void wait_words(const unsigned long long* p, long long stride, int n, uint32_t* v) {
+__device__ __forceinline__ void wait_words(const unsigned long long* p, long long stride, int n, uint32_t* v,
+                                           int* failed) {
   unsigned long long t0 = 0;
   unsigned have = 0;
   for (unsigned i = 0;; ++i) {
@@ -355,10 +371,10 @@ __device__ __forceinline__ void wait_words(const unsigned long long* p, long lon
     if ((i & 63) == 63) {
       const unsigned long long now = global_ns();
       if (!t0) t0 = now;
-      if (now - t0 > MBAR_WAIT_NS || timed_out(&g_moe_status)) break;
+      if (now - t0 > MBAR_WAIT_NS || timed_out(failed)) break;
     }
   }
-  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
+  wait_ran_out(failed);
 }
 
 __device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
@@ -406,26 +422,26 @@ struct Act {
 };
 
 // Waits until *p >= want, a second at most.
-__device__ __forceinline__ bool wait_count(const unsigned* p, unsigned want) {
+__device__ __forceinline__ bool wait_count(const unsigned* p, unsigned want, int* failed) {
   if (ld_acquire(p) >= want) return true;
   const unsigned long long t0 = global_ns();
   for (unsigned i = 0; i < MBAR_SPIN_LIMIT; ++i) {
     if (ld_acquire(p) >= want) return true;
-    if ((i & 63) == 63 && (global_ns() - t0 > MBAR_WAIT_NS || timed_out(&g_moe_status))) break;
+    if ((i & 63) == 63 && (global_ns() - t0 > MBAR_WAIT_NS || timed_out(failed))) break;
   }
-  atomicCAS(&g_moe_status, 0, ST_E_TIMEOUT);
+  wait_ran_out(failed);
   return false;
 }
 
 // The flags of blocks b0 to b1 of a group, by a warp; `all` once every tile's
 // flag is up, from when on there is nothing to wait for.
 __device__ __forceinline__ void wait_flags(const unsigned* flag, int b0, int b1, const unsigned* up_done, unsigned tiles,
-                                           bool* all) {
+                                           bool* all, int* failed) {
   if (*all) return;
   const int lane = threadIdx.x & 31;
   const unsigned v = ld_acquire(lane == 31 ? up_done : flag + min(b0 + lane, b1 - 1));
   *all = __shfl_sync(MS_FULL, v, 31) == tiles;
-  if (!*all && lane < 31 && v == 0) wait_count(flag + min(b0 + lane, b1 - 1), 1);
+  if (!*all && lane < 31 && v == 0) wait_count(flag + min(b0 + lane, b1 - 1), 1, failed);
   __syncwarp();
   fence_async_all();
 }
@@ -515,7 +531,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   Task* s_task = reinterpret_cast<Task*>(smem + C::OFF_TASK);             // [4]
   uint64_t* g_bar = t_empty + 4;                                          // [2] a group's warps meet
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(g_bar + 2);
-  int* const status = &g_moe_status;
+  int* const failed = w.failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int P = a.T * a.k;
 
@@ -584,11 +600,13 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (!shared_out) break;
     }
   }
+  bool lost = false;                        // the routing never came: this CTA takes no tasks
   if (shared_out) {
-    if (threadIdx.x == 0) wait_count(w.routed, (unsigned)a.T);
+    if (threadIdx.x == 0) s_word[0] = wait_count(w.routed, (unsigned)a.T, failed);
     __syncthreads();
-    for (int q = threadIdx.x; q < P; q += MOE_THREADS) {
-      const int t = q / a.k, at = t * 32 + q - t * a.k, e = __ldcg(w.inds + q) & 255;
+    lost = !s_word[0];
+    for (int q = threadIdx.x; q < P && !lost; q += MOE_THREADS) {
+      const int t = q / a.k, at = t * 32 + q - t * a.k, e = __ldcg(w.inds + q);
       s_prob[at] = __ldcg(w.probs + q);
       s_row[at] = (uint16_t)e;
       atomicOr(&s_mask[e], 1ull << t);
@@ -620,7 +638,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     if (lane == 0) s_word[warp - 4] = split;
   }
   __syncthreads();
-  for (int q = threadIdx.x; q < P; q += MOE_THREADS) {     // a choice's row, a row's token
+  for (int q = threadIdx.x; q < P && !lost; q += MOE_THREADS) {     // a choice's row, a row's token
     const int t = q / a.k, at = t * 32 + q - t * a.k, e = s_row[at];
     const int row = s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1));
     s_row[at] = (uint16_t)row;
@@ -632,7 +650,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
   sh.G = G, sh.S1 = ONE ? w.S1 : s_word[4], sh.S2 = ONE ? w.S2 : s_word[5];
   sh.FT = blocks128(a.f), sh.DT = blocks128(a.d), sh.KB1 = sh.DT, sh.KB2 = sh.FT;
   sh.n_up = sh.G * sh.FT * sh.S1, sh.n_dn = sh.G * sh.DT * sh.S2;
-  sh.n_co = sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
+  sh.n_co = lost ? 0 : sh.DT * ((a.T + COMBINE_T - 1) / COMBINE_T);
 
   // blocks of a down step
   auto down_per = [&](int g) { return __popcll(s_mask[s_group[g]]) <= 16 ? 2 : 1; };
@@ -644,7 +662,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     bool ok = true;
     int i = 0, n = 0;
     auto take = [&](unsigned id) {           // the n-th task, published to the other warps
-      if (n >= 4 && !mbar_wait_step(&t_empty[n & 3], ((n >> 2) - 1) & 1, status)) ok = false;
+      if (n >= 4 && !wait_step(&t_empty[n & 3], ((n >> 2) - 1) & 1, failed)) ok = false;
       const Task t = sh.task(ok ? id : 0xffffffffu);      // after a failure the other warps end
       if (lane == 0) {
         s_task[n & 3] = t;
@@ -661,7 +679,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     Task t = take(__shfl_sync(MS_FULL, first_task, 0));
     while (t.kind != 3) {
       if (t.kind == 2) {                     // one at a time, so that other CTAs take the next
-        if (!mbar_wait_step(&t_empty[(n - 1) & 3], ((n - 1) >> 2) & 1, status)) ok = false;
+        if (!wait_step(&t_empty[(n - 1) & 3], ((n - 1) >> 2) & 1, failed)) ok = false;
         t = take(ticket());
         continue;
       }
@@ -671,9 +689,9 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       const int e = s_group[t.g], per = t.kind == 0 ? 1 : down_per(t.g);
       for (int b = t.b0; b < t.b1 && ok; b += per, ++i) {
         const int s = i % C::STAGES;
-        if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
+        if (i >= C::STAGES && !wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, failed)) {
           // copies in flight land before the CTA ends
-          for (int j = i - C::STAGES; j < i && mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, status);) ++j;
+          for (int j = i - C::STAGES; j < i && mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr);) ++j;
           ok = false;
           break;
         }
@@ -704,7 +722,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     bool ok = true;
     int i = 0, c = 0, j0 = 0, j1 = 0;        // steps; compute tasks; steps of each group
     for (int n = 0; ok; ++n) {
-      if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
+      if (!wait_step(&t_full[n & 3], (n >> 2) & 1, failed)) break;
       const Task t = s_task[n & 3];
       __syncwarp();
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
@@ -716,8 +734,8 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int j = grp ? j1++ : j0++;
         const int s = i % C::STAGES, u = grp * C::BUFS + j % C::BUFS;
-        if (!mbar_wait_step(&full[s], (i / C::STAGES) & 1, status) ||
-            (j >= C::BUFS && !mbar_wait_step(&d_empty[u], ((j / C::BUFS) - 1) & 1, status))) {
+        if (!wait_step(&full[s], (i / C::STAGES) & 1, failed) ||
+            (j >= C::BUFS && !wait_step(&d_empty[u], ((j / C::BUFS) - 1) & 1, failed))) {
           ok = false;
           break;
         }
@@ -742,7 +760,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     bool ok = true, all_up = false;
     int i = 0;
     for (int n = 0; ok; ++n) {
-      if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
+      if (!wait_step(&t_full[n & 3], (n >> 2) & 1, failed)) break;
       const Task t = s_task[n & 3];
       __syncwarp();
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
@@ -759,12 +777,12 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
           for (int q = 0; q < MOE_FAC; ++q) v[q] = 0;
           // a lane's last block may lie beyond f
           const int at0 = t.b0 * 32 + lane, nb = t.b1 - t.b0 - (at0 + (t.b1 - t.b0 - 1) * 32 >= n4);
-          wait_words<MOE_FAC>(w.h_w + (long long)start * n4 + at0, 32, nb, v);
+          wait_words<MOE_FAC>(w.h_w + (long long)start * n4 + at0, 32, nb, v, failed);
 #pragma unroll
           for (int q = 0; q < MOE_FAC; q += 2) {
             if (t.b0 + q >= t.b1) break;
             const int s = i % C::STAGES;
-            if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
+            if (i >= C::STAGES && !wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, failed)) {
               ok = false;
               break;
             }
@@ -780,14 +798,14 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
       int tok[4];                            // up: the tokens of rows 4 lane to 4 lane + 3, none beyond the last
       if (t.kind == 1) {
-        wait_flags(w.flag + t.g * sh.FT, t.b0, t.b1, w.up_done, sh.G * sh.FT, &all_up);
+        wait_flags(w.flag + t.g * sh.FT, t.b0, t.b1, w.up_done, sh.G * sh.FT, &all_up, failed);
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q) tok[q] = 4 * lane + q < rows ? s_tok[start + 4 * lane + q] : a.T;
       }
       for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int s = i % C::STAGES;
-        if (i >= C::STAGES && !mbar_wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, status)) {
+        if (i >= C::STAGES && !wait_step(&empty[s], ((i / C::STAGES) - 1) & 1, failed)) {
           ok = false;
           break;
         }
@@ -811,7 +829,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     bool ok = true, all_up = false;
     int c = 0;
     for (int n = 0; ok; ++n) {
-      if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
+      if (!wait_step(&t_full[n & 3], (n >> 2) & 1, failed)) break;
       const Task t = s_task[n & 3];
       __syncwarp();
       if (lane == 0) mbar_arrive1(&t_empty[n & 3]);
@@ -825,7 +843,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       if (t.kind == 0) {
         const long long at = ((long long)e * sh.FT + t.tile) * sh.KB1 + b;
         const float wg = __ldg(a.gate.s + at), wu = __ldg(a.up.s + at);
-        if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
+        if (c >= 2) ok = wait_step(&f_empty[u], ((c >> 1) - 1) & 1, failed);
 #pragma unroll 8
         for (int r = r0; r < rows; r += 2) {
           const float x = __ldcg(w.xs + s_tok[start + r] * sh.KB1 + b);
@@ -835,17 +853,17 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         const float wd = __ldg(a.down.s + ((long long)e * sh.DT + t.tile) * sh.KB2 + b);
         if constexpr (ONE) {
           uint32_t x;
-          wait_words<1>(w.hs_w + (long long)start * sh.KB2 + b, 0, 1, &x);
+          wait_words<1>(w.hs_w + (long long)start * sh.KB2 + b, 0, 1, &x, failed);
           __syncwarp();
-          if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
+          if (c >= 2) ok = wait_step(&f_empty[u], ((c >> 1) - 1) & 1, failed);
           if (lane < nb) fac[0] = __uint_as_float(x) * wd;
           ++c;
           __syncwarp();
           if (lane == 0) mbar_arrive1(&f_full[u]);
           continue;
         }
-        wait_flags(w.flag + t.g * sh.FT, t.b0, t.b1, w.up_done, sh.G * sh.FT, &all_up);
-        if (c >= 2) ok = mbar_wait_step(&f_empty[u], ((c >> 1) - 1) & 1, status);
+        wait_flags(w.flag + t.g * sh.FT, t.b0, t.b1, w.up_done, sh.G * sh.FT, &all_up, failed);
+        if (c >= 2) ok = wait_step(&f_empty[u], ((c >> 1) - 1) & 1, failed);
 #pragma unroll 8
         for (int r = r0; r < rows; r += 2) {
           const float x = __ldcg(w.hs + (long long)(start + r) * sh.KB2 + b);
@@ -875,14 +893,14 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     auto meet = [&] {
       __syncwarp();
       if (lane == 0) mbar_arrive1(&g_bar[grp]);
-      if (!mbar_wait_step(&g_bar[grp], met & 1, status)) ok = false;
+      if (!wait_step(&g_bar[grp], met & 1, failed)) ok = false;
       ++met;
     };
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float* s_rows = reinterpret_cast<float*>(smem + C::OFF_ROWS) + grp * (2 * MOE_ROWS * 128);
     float acc[2][NT];
     for (int n = 0; ok; ++n) {
-      if (!mbar_wait_step(&t_full[n & 3], (n >> 2) & 1, status)) break;
+      if (!wait_step(&t_full[n & 3], (n >> 2) & 1, failed)) break;
       const Task t = s_task[n & 3];
       __syncwarp();
       const bool combine = t.kind == 2 && grp == 0;
@@ -894,7 +912,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         // y of four tokens, one per warp: rows in the order of the token's
         // choices, ranges in order
         if (!ONE) {
-          if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2 * 4));
+          if (tid == 0) wait_count(w.dn_done + t.tile, (unsigned)(sh.G * sh.S2 * 4), failed);
           meet();
         }
         const int f = t.tile * 128 + lane * 4, tok = t.s * COMBINE_T + warp;
@@ -915,7 +933,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
 #pragma unroll
                   for (int j = 0; j < 4; ++j)
                     p[j] = w.dn_w + (long long)(r0 + s_row[min(j0 + 4 * h + j, a.k - 1)]) * a.d + f;
-                  wait_quads(p, v);
+                  wait_quads(p, v, failed);
 #pragma unroll
                   for (int j = 0; j < 4; ++j) {
                     o[4 * h + j].x += __uint_as_float(v[j][0]), o[4 * h + j].y += __uint_as_float(v[j][1]);
@@ -961,7 +979,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       const int e = s_group[t.g], start = s_start[e];
       const int rows = __popcll(s_mask[e]);
       const float* fac = s_fac + grp * (MOE_FAC * 2 * NT);
-      ok = mbar_wait_step(&f_full[grp], (c >> 1) & 1, status);
+      ok = wait_step(&f_full[grp], (c >> 1) & 1, failed);
 #pragma unroll
       for (int m = 0; m < NT; ++m) acc[0][m] = acc[1][m] = 0.f;
       auto take = [&](float* sum, uint32_t at, const float* f) {
@@ -988,7 +1006,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       };
       for (int b = t.b0; b < t.b1; b += per, ++i) {
         const int u = grp * C::BUFS + i % C::BUFS;
-        if (!ok || !mbar_wait_step(&d_full[u], (i / C::BUFS) & 1, status)) {
+        if (!ok || !wait_step(&d_full[u], (i / C::BUFS) & 1, failed)) {
           ok = false;
           break;
         }
@@ -1038,7 +1056,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
             put_word(word + (2 * t.s + 1) * stride, __float_as_uint(acc[1][0]));
           } else if (sh.S1 > 1) {
             uint32_t v[2 * (MOE_SPLIT - 1)];
-            wait_words<2 * (MOE_SPLIT - 1)>(word, stride, 2 * (sh.S1 - 1), v);
+            wait_words<2 * (MOE_SPLIT - 1)>(word, stride, 2 * (sh.S1 - 1), v, failed);
             float g = 0.f, u = 0.f;
 #pragma unroll
             for (int q = 0; q < MOE_SPLIT - 1; ++q)
@@ -1192,6 +1210,19 @@ cudaError_t launch_moe_fp8(const MoeFp8Args& a, int sms, cudaStream_t s) {
   if (a.T <= 16) return launch_experts<16, false>(a, w, sms, s);
   if (a.T <= 32) return launch_experts<32, false>(a, w, sms, s);
   return launch_experts<64, false>(a, w, sms, s);
+}
+
+// The experts' kernel over a workspace in which no token is ever routed: every
+// CTA's wait for the routing runs out after its second.
+cudaError_t launch_moe_fp8_lost(const MoeFp8Args& a, int sms, cudaStream_t s) {
+  MoeWs w;
+  layout_ws(a.ws, a.T, a.d, a.f, a.E, a.k, sms, &w);
+  cudaError_t e = cudaMemsetAsync(w.next, 0, 4ll * w.counters, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(w.rt_next, 0x7f, 4, s);     // beyond the last token
+  if (e != cudaSuccess) return e;
+  return a.T <= 16   ? launch_experts<16, false>(a, w, sms, s)
+         : a.T <= 32 ? launch_experts<32, false>(a, w, sms, s)
+                     : launch_experts<64, false>(a, w, sms, s);
 }
 
 cudaError_t moe_fp8_status(int** at) { return cudaGetSymbolAddress(reinterpret_cast<void**>(at), g_moe_status); }
