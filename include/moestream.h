@@ -481,8 +481,10 @@ int ms_moe_fp8_layer(const ms_fp8_moe* args, void* stream);
 
 /* Sticky device-side status of the fp8 operators on `device`: MS_OK, or
  * MS_E_TIMEOUT when a bounded wait inside one of their kernels ran out (that
- * call's output is not valid). Also written to *status; reading clears it.
- * Waits for `stream`; not for use in a capture. */
+ * call's output is not valid; other calls are not affected). Also written to
+ * *status; reading clears it, in one step with the reading. Waits for `stream`,
+ * MS_HOST_WAIT_S at most: MS_E_TIMEOUT with *status MS_OK when it has not
+ * finished by then. Refused in a capture. */
 int ms_fp8_status(int device, int* status, void* stream);
 
 /* Failure-detection self-test, no reference counterpart: ms_moe_fp8_layer's

@@ -1,8 +1,9 @@
 // Entry points of the fp8 operators (include/moestream.h): argument checks
-// and launches. Nothing here allocates, synchronises (but for ms_fp8_status)
-// or throws.
+// and launches. Nothing here allocates or synchronises, but for ms_fp8_status,
+// which waits for a stream and keeps a few pinned words, and nothing throws.
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "../../include/moestream.h"
 #include "fp8.cuh"
@@ -179,6 +180,45 @@ extern "C" int ms_fp8_selftest_wait(const ms_fp8_moe* p, void* stream) {
   return moe_call(me, p, stream, launch_moe_fp8_lost);
 }
 
+namespace {
+
+// Reads and clears both words in one step each: what a kernel on another
+// stream records is either in this answer or left for the next.
+__global__ void k_take_status(int* linear, int* moe, volatile int* answer) {
+  answer[0] = atomicExch(linear, 0);
+  answer[1] = atomicExch(moe, 0);
+}
+
+// Pinned words for an answer, kept from call to call: two ints each, mapped on
+// every device. Those of a call that gave up waiting are not used again, as
+// its kernel may yet write them.
+std::mutex g_answers_mutex;
+int* g_answers[16];
+int g_n_answers = 0;
+
+int* take_answer() {
+  {
+    std::lock_guard<std::mutex> lock(g_answers_mutex);
+    if (g_n_answers) return g_answers[--g_n_answers];
+  }
+  void* p = nullptr;
+  if (cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) return static_cast<int*>(p);
+  cudaGetLastError();
+  return nullptr;
+}
+void give_answer(int* a) {
+  {
+    std::lock_guard<std::mutex> lock(g_answers_mutex);
+    if (g_n_answers < 16) {
+      g_answers[g_n_answers++] = a;
+      return;
+    }
+  }
+  cudaFreeHost(a);
+}
+
+}  // namespace
+
 extern "C" int ms_fp8_status(int device, int* status, void* stream) {
   const char* me = "ms_fp8_status";
   if (!status) return bad(MS_E_INVALID, "%s: status is NULL", me);
@@ -186,21 +226,32 @@ extern "C" int ms_fp8_status(int device, int* status, void* stream) {
   OnDevice on(device);
   if (on.err != cudaSuccess) return bad(MS_E_CUDA, "%s: device %d: %s", me, device, cudaGetErrorString(on.err));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int *at[2] = {}, st[2] = {};
+  cudaStreamCaptureStatus capturing;
+  cudaError_t e = cudaStreamIsCapturing(s, &capturing);
+  if (e != cudaSuccess || capturing != cudaStreamCaptureStatusNone)
+    return bad(MS_E_INVALID, "%s: not for use in a capture", me);
+  int* at[2] = {};
   if (linear_fp8_status(&at[0]) != cudaSuccess || moe_fp8_status(&at[1]) != cudaSuccess)
     return bad(MS_E_CUDA, "%s: the status words have no address", me);
-  for (int i = 0; i < 2; ++i)
-    if (cudaMemcpyAsync(&st[i], at[i], sizeof(int), cudaMemcpyDeviceToHost, s) != cudaSuccess)
-      return bad(MS_E_CUDA, "%s: reading the status failed", me);
-  cudaError_t e = stream_wait_bounded(s);
+  // The stream's work first: while it has not finished, nothing is taken.
+  e = stream_wait_bounded(s);
+  int st[2] = {};
+  if (e == cudaSuccess) {
+    int* answer = take_answer();
+    if (!answer) return bad(MS_E_CUDA, "%s: no pinned memory for the answer", me);
+    k_take_status<<<1, 1, 0, s>>>(at[0], at[1], answer);
+    e = cudaGetLastError();
+    const bool asked = e == cudaSuccess;
+    if (asked) e = stream_wait_bounded(s);
+    if (e == cudaSuccess) {
+      const volatile int* v = answer;
+      st[0] = v[0], st[1] = v[1];
+    }
+    if (e == cudaSuccess || !asked) give_answer(answer);
+  }
   if (e == cudaErrorTimeout)
     return bad(MS_E_TIMEOUT, "%s: the stream did not finish within the host wait limit (MS_HOST_WAIT_S)", me);
   if (e != cudaSuccess) return bad(MS_E_CUDA, "%s: %s", me, cudaGetErrorString(e));
   *status = st[0] ? st[0] : st[1];
-  if (*status == MS_OK) return MS_OK;
-  for (int i = 0; i < 2; ++i)
-    if (cudaMemsetAsync(at[i], 0, sizeof(int), s) != cudaSuccess)
-      return bad(MS_E_CUDA, "%s: clearing the status failed", me);
-  if (stream_wait_bounded(s) != cudaSuccess) return bad(MS_E_CUDA, "%s: clearing the status failed", me);
-  return bad(*status, "an fp8 operator's bounded wait ran out: its output is not valid");
+  return *status == MS_OK ? MS_OK : bad(*status, "an fp8 operator's bounded wait ran out: its output is not valid");
 }
