@@ -238,11 +238,24 @@ def _weight(name, codes, scales, rank, device=None):
     return codes, scales.contiguous()
 
 
+def _wait_for_copies(device, given, used):
+    """Calls may come on any stream, so the copies that a constructor has
+    queued are waited for. Inside a capture they are part of the graph, and so
+    are the calls that may read them."""
+    if any(u is not None and u.data_ptr() != g.data_ptr() for g, u in zip(given, used)):
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
+
+
 class Fp8Linear:
     """y = x w^T (+ bias) for a weight w [N, K] in codes and block scales.
 
     A weight whose rows are contiguous and start on 16-byte boundaries is used
-    where it is; another is copied once, here."""
+    where it is; another is copied once, here, as are scales that are not
+    contiguous and a bias that is not float32. The copies are waited for, so
+    the layer may be called on any stream; a layer that copies inside a capture
+    belongs to that graph."""
 
     def __init__(self, weight, scales, bias=None):
         w, self.scales = _weight("weight", weight, scales, 2)
@@ -256,6 +269,7 @@ class Fp8Linear:
         self.weight = w
         self.bias = _bias(bias, (N,), w.device)
         self.device = w.device
+        _wait_for_copies(w.device, (weight, scales, bias), (w, self.scales, self.bias))
         self._w = (w.data_ptr(), self.scales.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
         self._ld = _row_stride(w)
         self._dims = (K, N, _blocks(K), w.get_device())
@@ -313,7 +327,9 @@ class Fp8MoELayer:
     SwiGLU). router: bf16 [E, d] (and router_bias [E]); gate, up: (codes
     [E, f, d], scales[, bias [E, f]]); down: (codes [E, d, f], scales[, bias
     [E, d]]). d and f are multiples of 16. The logits are kept in 32 bits
-    (MoEBlock rounds them to bf16 as the reference does)."""
+    (MoEBlock rounds them to bf16 as the reference does). Weights that are
+    contiguous and 16-byte aligned are used where they are; copies are made and
+    waited for as Fp8Linear's."""
 
     def __init__(self, model, router, gate, up, down, top_k, router_bias=None, norm_topk_prob=True):
         if model not in ("qwen3", "gptoss"):
@@ -341,6 +357,9 @@ class Fp8MoELayer:
                 raise ValueError(f"{name} has shape {tuple(codes.shape)}, expected {(E, n, k)}")
             parts.append((self._aligned(codes), scales, _bias(m[2] if len(m) > 2 else None, (E, n), self.device)))
         self.gate, self.up, self.down = parts
+        given = [t for m in (gate, up, down) for t in (*m[:2], m[2] if len(m) > 2 else None)]
+        _wait_for_copies(self.device, (router, router_bias, *given),
+                         (self.router, self.router_bias, *(t for p in parts for t in p)))
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         self._ptrs = (*(ptr(p[0]) for p in parts), *(ptr(p[1]) for p in parts), *(ptr(p[2]) for p in parts))
         self._router = (ptr(self.router), ptr(self.router_bias))
