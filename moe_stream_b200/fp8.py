@@ -17,7 +17,7 @@ code times scale is the value). The quantiser's scales are powers of two; the
 products take any scale.
 
 Everything is asynchronous on the current stream of the inputs' device (or on
-``stream=``), allocates only through torch, keeps no state between calls and
+``stream=``, which the caller has made to wait for the inputs), allocates only through torch, keeps no state between calls and
 can be captured into a CUDA graph. As in the rest of the package there is no
 CPU implementation and no backward pass.
 """
@@ -49,13 +49,19 @@ def _stream(device, stream=None):
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
-def _on_stream(call, stream, device, *args):
+def _on_stream(call, stream, device, *args, keep=()):
     """call(*args) with `stream` current: the tensors it makes belong to the
-    stream that writes them."""
+    stream that writes them. The tensors it reads (args, and `keep`) may be
+    dropped once it returns: their memory is not used again before `stream`
+    has come past the call."""
     if stream.device.index != device:
         raise ValueError(f"stream is on {stream.device}, the inputs on cuda:{device}")
     with torch.cuda.stream(stream):
-        return call(*args)
+        out = call(*args)
+    for t in (*args, *keep):
+        if isinstance(t, torch.Tensor):
+            t.record_stream(stream)
+    return out
 
 
 def _rows(name, t, d=None, dtype=None):
@@ -279,7 +285,8 @@ class Fp8Linear:
         """[..., N] of codes q [..., K] and scales [..., ceil(K/128)], in
         bf16, fp16 or fp32."""
         if stream is not None:
-            return _on_stream(self._forward, stream, self.device.index, q, scales, out_dtype, out)
+            return _on_stream(self._forward, stream, self.device.index, q, scales, out_dtype, out,
+                              keep=(self.weight, self.scales, self.bias))
         return self._forward(q, scales, out_dtype, out)
 
     def _forward(self, q, scales, out_dtype, out):
@@ -387,7 +394,8 @@ class Fp8MoELayer:
         """x [..., d] bf16 -> y [..., d] bf16, residual (like x) added. out
         may be x or residual."""
         if stream is not None:
-            return _on_stream(self._forward, stream, self.device.index, x, residual, out)
+            return _on_stream(self._forward, stream, self.device.index, x, residual, out,
+                              keep=(self.router, self.router_bias, *self.gate, *self.up, *self.down))
         return self._forward(x, residual, out)
 
     def _forward(self, x, residual, out):

@@ -81,3 +81,53 @@ def test_constructors_in_a_capture(lib, cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+def test_tensors_dropped_after_the_call(lib, cuda):
+    """Inputs and layers that are dropped as soon as a call on a stream that is
+    held up returns: their memory is not used again before it has run."""
+    from moe_stream_b200 import fp8
+    g = _gen(3)
+    T, d, N = 61, 2048, 1536
+    side = torch.cuda.Stream()
+    x0, r0 = (torch.randn(T, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    n0 = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(torch.bfloat16)
+    q0, s0 = fp8.quantize_fp8(x0)
+    w0, ws0 = _weight(g, N, d)
+    router, parts = _moe(g)
+    y0 = torch.randn(T, 256, generator=g, device="cuda").to(torch.bfloat16)
+
+    def norm():
+        x, n, r = x0.clone(), n0.clone(), r0.clone()
+        return lambda **kw: fp8.rms_norm_fp8(x, n, residual=r, **kw)
+
+    def quantize():
+        x = x0.clone()
+        return lambda **kw: fp8.quantize_fp8(x, **kw)
+
+    def linear():
+        layer, q, s = fp8.Fp8Linear(w0.clone(), ws0.clone()), q0.clone(), s0.clone()
+        return lambda **kw: (layer(q, s, **kw),)
+
+    def moe():
+        layer = fp8.Fp8MoELayer("qwen3", router.clone(), *[tuple(t.clone() for t in p) for p in parts], top_k=2)
+        y, r = y0.clone(), y0.clone()
+        return lambda **kw: (layer(y, residual=r, **kw),)
+
+    for make in (norm, quantize, linear, moe):
+        want = make()()
+        torch.cuda.synchronize()
+        call = make()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(DELAY)
+        got = call(stream=side)
+        del call
+        # whatever was freed is taken and spoilt, on this stream, at once
+        spoilt = [torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda")
+                  for n in (512, 2048, 4096, 2 * T * d, T * d, N * d, 4 * ws0.numel(), 8 * 384 * 256, 2 * T * 256,
+                            2 * router.numel(), 2 * 8 * 384, 4 * 8 * 384, 4 * s0.numel()) for _ in range(6)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), make.__name__
+        del spoilt, got, want
