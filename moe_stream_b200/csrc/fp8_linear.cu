@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(FEW_THREADS)
   uint64_t* d_empty = d_full + C::BUFS;      // [BUFS]   taken out
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(d_empty + C::BUFS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = gridDim.x, rank = blockIdx.x;
-  const int n0 = blockIdx.y * 128, m0 = blockIdx.z * NT;
+  const int split = cluster_size(), rank = cluster_rank(), tile = cluster_id();
+  const int n0 = tile * 128, m0 = blockIdx.y * NT;
   const int kb = (a.K + 127) / 128;
   const int b0 = (int)((long long)kb * rank / split), b1 = (int)((long long)kb * (rank + 1) / split);
 
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
     }
   } else {
     grid_wait();
-    const float* ws = a.ws + (long long)blockIdx.y * kb;
+    const float* ws = a.ws + (long long)tile * kb;
     bool ok = true;
     // after a wait that ran out the warp goes on to the barriers, without the
     // products: others may be waiting there
@@ -553,7 +553,7 @@ static cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s) {
   cudaError_t e = allow_shared<k_linear_few<NT, OUT>>(Few<NT>::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(split, tiles, cols);
+  cfg.gridDim = dim3(split * tiles, cols);       // x alone goes beyond 65535
   cfg.blockDim = dim3(FEW_THREADS);
   cfg.dynamicSmemBytes = Few<NT>::SMEM;
   cfg.stream = s;

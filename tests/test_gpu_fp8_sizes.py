@@ -1,0 +1,33 @@
+"""The fp8 operators at the ends of their sizes."""
+import pytest
+import torch
+
+from oracle import fp8 as O
+
+pytestmark = pytest.mark.gpu
+
+
+def _codes(g, n, k):
+    """Random codes without a NaN, in rows of 16 bytes or a multiple."""
+    c = torch.randint(0, 0x60, (n, (k + 15) // 16 * 16), generator=g, device="cuda", dtype=torch.uint8)
+    c[:, ::3] |= 0x80
+    return c.view(torch.float8_e4m3fn)[:, :k]
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 64])
+@pytest.mark.parametrize("N,K", [(65535 * 128 + 130, 16), (65536 * 128, 130), (2 * 65536 * 128 + 1, 5)])
+def test_linear_of_very_many_outputs(M, N, K, lib, cuda):
+    """More than 65535 tiles of outputs for a few rows."""
+    from moe_stream_b200 import fp8
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    kb = -(-K // 128)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    xs = torch.rand(M, kb, generator=g, device="cuda") + 0.5
+    ws = (torch.rand(-(-N // 128), kb, generator=g, device="cuda") + 0.5) * 2.0 ** -12
+    y = fp8.Fp8Linear(w, ws)(x, xs)
+    assert y.shape == (M, N)
+    for n in (0, 65535 * 128 - 128, 65535 * 128, (N - 1) // 128 * 128):
+        part = slice(n, min(N, n + 128))
+        want, tol = O.product(O.rows_value(x, xs), O.weight_value(w[part], ws[n // 128:n // 128 + 1]), kb)
+        lim = tol + 2.0 ** -8 * (want.abs() + tol)
+        assert ((y[:, part].double() - want).abs() <= lim).all(), n
