@@ -407,6 +407,7 @@ int ms_expert_mlp_static_status(void* stream);
 #define MS_DT_F32         2
 #define MS_FP8_MAX_FEATURES 16384
 #define MS_FP8_MAX_TOKENS 64
+#define MS_FP8_MAX_ROWS 2147418112   /* 2^31 - 2^16: of T, M, N and K, whose tiles are counted in 32 bits */
 
 /* Residual add, RMSNorm and quantisation (the norm and residual of
  * ms_moe_block_fused, with an 8-bit output), per row of d features:

@@ -61,7 +61,7 @@ int launched(const char* what, cudaError_t e) {
 extern "C" int ms_rms_norm_fp8(const ms_fp8_norm* p, void* stream) {
   const char* me = "ms_rms_norm_fp8";
   if (!p) return bad(MS_E_INVALID, "%s: the argument block is NULL", me);
-  if (p->T < 0) return bad(MS_E_INVALID, "%s: T must not be negative", me);
+  if (p->T < 0 || p->T > MS_FP8_MAX_ROWS) return bad(MS_E_INVALID, "%s: T must be in [0, %d]", me, MS_FP8_MAX_ROWS);
   if (p->T == 0) return MS_OK;
   if (!p->x || !p->q || !p->scales) return bad(MS_E_INVALID, "%s: x, q or scales is NULL", me);
   if (p->d < 1 || p->d > MS_FP8_MAX_FEATURES)
@@ -88,11 +88,12 @@ extern "C" int ms_rms_norm_fp8(const ms_fp8_norm* p, void* stream) {
 extern "C" int ms_linear_fp8(const ms_fp8_linear* p, void* stream) {
   const char* me = "ms_linear_fp8";
   if (!p) return bad(MS_E_INVALID, "%s: the argument block is NULL", me);
-  if (p->M < 0) return bad(MS_E_INVALID, "%s: M must not be negative", me);
+  if (p->M < 0 || p->M > MS_FP8_MAX_ROWS) return bad(MS_E_INVALID, "%s: M must be in [0, %d]", me, MS_FP8_MAX_ROWS);
   if (p->M == 0) return MS_OK;
   if (!p->x || !p->x_scales || !p->w || !p->w_scales || !p->y)
     return bad(MS_E_INVALID, "%s: x, w, their scales or y is NULL", me);
-  if (p->N < 1 || p->K < 1) return bad(MS_E_INVALID, "%s: N and K must be positive", me);
+  if (p->N < 1 || p->K < 1 || p->N > MS_FP8_MAX_ROWS || p->K > MS_FP8_MAX_ROWS)
+    return bad(MS_E_INVALID, "%s: N and K must be in [1, %d]", me, MS_FP8_MAX_ROWS);
   if (p->out_dtype < MS_DT_BF16 || p->out_dtype > MS_DT_F32)
     return bad(MS_E_INVALID, "%s: unknown out_dtype %d", me, p->out_dtype);
   if (off16(p->x) || off16(p->w) || p->x_stride % 16 || p->w_stride % 16)

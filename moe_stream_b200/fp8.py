@@ -31,6 +31,7 @@ from . import _lib
 BLOCK = 128
 MAX_TOKENS = 64           # MS_FP8_MAX_TOKENS
 MAX_FEATURES = 16384      # MS_FP8_MAX_FEATURES
+MAX_ROWS = 2 ** 31 - 2 ** 16   # MS_FP8_MAX_ROWS
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _E4M3 = torch.float8_e4m3fn
 
@@ -132,6 +133,8 @@ def _norm_call(x, weight, eps, residual, h_out, with_norm):
     if not 1 <= d <= MAX_FEATURES:
         raise ValueError(f"x has {d} features, supported are 1 to {MAX_FEATURES}")
     T = x.numel() // d
+    if T > MAX_ROWS:
+        raise ValueError(f"x has {T} rows, at most {MAX_ROWS} per call")
     dev = x.get_device()
     wp = rp = hp = yp = rs = 0
     h = y = None
@@ -268,6 +271,8 @@ class Fp8Linear:
         self.out_features, self.in_features = N, K = w.shape
         if N < 1 or K < 1:
             raise ValueError("weight must not be empty")
+        if max(N, K) > MAX_ROWS:
+            raise ValueError(f"weight has {N} rows of {K}, supported are {MAX_ROWS} of either")
         if (K > 1 and w.stride(1) != 1) or w.data_ptr() % 16 or _row_stride(w) % 16 or _row_stride(w) < K:
             p = _codes_like((N,), K, w.device)
             p.copy_(w)
@@ -302,6 +307,8 @@ class Fp8Linear:
         x = _rows("codes", q, K, _E4M3)
         s = _rows("scales", scales, KB, torch.float32)
         M, ld, ls = x.shape[0], (K + 15) // 16 * 16, KB
+        if M > MAX_ROWS:
+            raise ValueError(f"codes have {M} rows, at most {MAX_ROWS} per call")
         if M > 1:
             ld, ls = x.stride(0), s.stride(0)
             if ls < KB:

@@ -31,3 +31,21 @@ def test_linear_of_very_many_outputs(M, N, K, lib, cuda):
         want, tol = O.product(O.rows_value(x, xs), O.weight_value(w[part], ws[n // 128:n // 128 + 1]), kb)
         lim = tol + 2.0 ** -8 * (want.abs() + tol)
         assert ((y[:, part].double() - want).abs() <= lim).all(), n
+
+
+def test_row_counts_beyond_the_limit(lib, cuda):
+    """2^31 rows and those just below are refused, by expanded tensors that
+    hold one row."""
+    from moe_stream_b200 import fp8
+    one = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    q, s = fp8.quantize_fp8(one)
+    w = torch.zeros(16, 1, device="cuda").to(torch.float8_e4m3fn)
+    lin = fp8.Fp8Linear(w, torch.ones(1, 1, device="cuda"))
+    for T in (1 << 31, (1 << 31) - 1, (1 << 31) - (1 << 16) + 1):
+        for bad in (lambda: fp8.quantize_fp8(one.expand(T, 1)), lambda: fp8.rms_norm_fp8(one.expand(T, 1), one[0]),
+                    lambda: lin(q.expand(T, 1), s.expand(T, 1)),
+                    lambda: fp8.Fp8Linear(w[:1].expand(T, 1), torch.ones(1, 1, device="cuda").expand(-(-T // 128), 1))):
+            with pytest.raises(ValueError, match="rows"):
+                bad()
+    q2, s2 = fp8.quantize_fp8(one)
+    assert torch.equal(q2.double(), q.double()) and torch.equal(s2, s)
