@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(FEW_THREADS)
         const uint64_t ad = k128_desc(smem + s * C::STAGE), bd = k128_desc(smem + s * C::STAGE + FP8_W_TILE);
 #pragma unroll
         for (int j = 0; j < 4; ++j) mma_e4m3(tmem + u * NT, ad + 2 * j, bd + 2 * j, idesc, j != 0);
-        mma_done(&empty[s]);
+        // no report that nobody waits for: it might come after the CTA's end
+        if (b + C::STAGES < b1) mma_done(&empty[s]);
         mma_done(&d_full[u]);
       }
       __syncwarp();
@@ -331,6 +332,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1)
           __syncwarp();
         }
       }
+      if (ok) mbar_wait_ring<STAGES>(empty, i, &g_linear_status);
     } else if (warp == 9 && rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3(TM, TN);
       bool ok = true;

@@ -81,6 +81,18 @@ __device__ __forceinline__ bool mbar_wait_step(uint64_t* bar, unsigned phase, in
   return mbar_wait(bar, phase, status);
 }
 
+// By a warp, a lane per stage: a ring of N stages of which `used` have been
+// filled is given back whole. An MMA's report to a stage's barrier is still on
+// its way when its product can be read, and the barrier has to be there until
+// it has come. (A loop over the stages took a single token's MoE layer from 18.8
+// to 19.3 us; by lanes it is within 0.1 us.)
+template <int N>
+__device__ __forceinline__ void mbar_wait_ring(uint64_t* empty, int used, int* status) {
+  const int j = used - 1 - (int)(threadIdx.x & 31);
+  if (j >= 0 && j >= used - N) mbar_wait_step(&empty[j % N], (j / N) & 1, status);
+  __syncwarp();
+}
+
 __device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }

@@ -715,6 +715,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       }
       t = next;
     }
+    if (ok) mbar_wait_ring<C::STAGES>(empty, i, nullptr);
   } else if (warp == 5) {
     // ---- MMAs. Each group has buffers of its own and meets every phase of
     // their barriers in turn: a wait for a parity does not tell a phase from
