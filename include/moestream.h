@@ -462,8 +462,9 @@ int ms_linear_fp8(const ms_fp8_linear* args, void* stream);
  *   y = sum_j p_j (down product_j (+ bias)) (+ residual), bf16.
  * codes, scales, bias: gate, up [n_experts][d_ff][d_model] and down
  * [n_experts][d_model][d_ff], contiguous. y may be x or residual. workspace:
- * ms_moe_fp8_workspace bytes of device memory (it reads the sizes alone), for
- * this call alone until it has run; it needs no initialisation. */
+ * ms_moe_fp8_workspace bytes of device memory (it reads the sizes alone; up to 3
+ * GB at the largest sizes), for this call alone until it has run; it needs no
+ * initialisation. */
 typedef struct ms_fp8_moe {
   const void* x;            /* bf16 [T, d_model]                                   */
   const void* router;       /* bf16 [n_experts, d_model]                           */

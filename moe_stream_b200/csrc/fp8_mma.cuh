@@ -24,14 +24,7 @@ __device__ __forceinline__ void tma_tile_2d(void* dst, const CUtensorMap* tm, in
       "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tma_tile_3d(void* dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-// tma_tile_3d of data that is read once: its lines leave L2 first
+// of data that is read once: its lines leave L2 first
 __device__ __forceinline__ void tma_tile_3d_once(void* dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar,
                                                  uint64_t policy) {
   asm volatile(

@@ -72,9 +72,11 @@ static_assert(MOE_THREADS / 32 == MOE_FP8_ROUTED_HERE, "a warp per token");
 __host__ __device__ inline int blocks128(int n) { return (n + 127) / 128; }
 inline long long up16(long long n) { return (n + 15) / 16 * 16; }
 
-// Ranges that a tile's blocks may be cut into: enough for a task's scales to
-// fit and for few tiles to fill the GPU, while the sums in the workspace stay
-// below 64 MB a matrix.
+// Ranges that a tile's blocks may be cut into at most: as many as a task's
+// scales need to fit (a range of 16 blocks), two in any case, and up to eight,
+// so that few tiles fill the GPU, while the sums in the workspace stay below 64
+// MB a matrix. The first two go before the 64 MB: 64 tokens of 32 choices with
+// d and f 16384 take 2 GB for gate and up and 1 GB for down.
 inline int split_cap(long long pairs, int n, int kb) {
   const long long fit = (64ll << 20) / (pairs * n * 4);
   const int least = (kb + MOE_FAC - 1) / MOE_FAC;
@@ -613,38 +615,38 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     }
   }
   if constexpr (!ONE) {
-  __syncthreads();
-  // groups: the experts that have rows, ascending; their rows follow each other
-  const int mine_n = threadIdx.x < 256 ? __popcll(s_mask[threadIdx.x]) : 0;
-  G = __syncthreads_count(mine_n > 0);
-  if (warp < 8) {                           // rows in the low half, groups in the high; sums of the warps before
-    int at = mine_n + (mine_n ? 1 << 16 : 0);
+    __syncthreads();
+    // groups: the experts that have rows, ascending; their rows follow each other
+    const int mine_n = threadIdx.x < 256 ? __popcll(s_mask[threadIdx.x]) : 0;
+    G = __syncthreads_count(mine_n > 0);
+    if (warp < 8) {                           // rows in the low half, groups in the high; sums of the warps before
+      int at = mine_n + (mine_n ? 1 << 16 : 0);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(MS_FULL, at, o);
-      if (lane >= o) at += u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(MS_FULL, at, o);
+        if (lane >= o) at += u;
+      }
+      if (lane == 31) s_word[8 + warp] = at;
+      named_bar(1, 256);
+      for (int q = 0; q < warp; ++q) at += s_word[8 + q];
+      if (mine_n) {
+        s_group[(at >> 16) - 1] = (uint8_t)threadIdx.x;
+        s_start[threadIdx.x] = (at & 0xffff) - mine_n;
+      }
+    } else if (warp < 10) {
+      const int nf = blocks128(a.f), nd = blocks128(a.d);
+      const int split = warp == 8 ? choose_split(G * nf, nd, gridDim.x, w.cap1, 2.f)
+                                  : choose_split(G * nd, nf, gridDim.x, w.cap2, 0.5f);
+      if (lane == 0) s_word[warp - 4] = split;
     }
-    if (lane == 31) s_word[8 + warp] = at;
-    named_bar(1, 256);
-    for (int q = 0; q < warp; ++q) at += s_word[8 + q];
-    if (mine_n) {
-      s_group[(at >> 16) - 1] = (uint8_t)threadIdx.x;
-      s_start[threadIdx.x] = (at & 0xffff) - mine_n;
+    __syncthreads();
+    for (int q = threadIdx.x; q < P && !lost; q += MOE_THREADS) {     // a choice's row, a row's token
+      const int t = q / a.k, at = t * 32 + q - t * a.k, e = s_row[at];
+      const int row = s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1));
+      s_row[at] = (uint16_t)row;
+      s_tok[row] = (uint8_t)t;
     }
-  } else if (warp < 10) {
-    const int nf = blocks128(a.f), nd = blocks128(a.d);
-    const int split = warp == 8 ? choose_split(G * nf, nd, gridDim.x, w.cap1, 2.f)
-                                : choose_split(G * nd, nf, gridDim.x, w.cap2, 0.5f);
-    if (lane == 0) s_word[warp - 4] = split;
-  }
-  __syncthreads();
-  for (int q = threadIdx.x; q < P && !lost; q += MOE_THREADS) {     // a choice's row, a row's token
-    const int t = q / a.k, at = t * 32 + q - t * a.k, e = s_row[at];
-    const int row = s_start[e] + __popcll(s_mask[e] & ((1ull << t) - 1));
-    s_row[at] = (uint16_t)row;
-    s_tok[row] = (uint8_t)t;
-  }
-  __syncthreads();
+    __syncthreads();
   }
   Shape sh;
   sh.G = G, sh.S1 = ONE ? w.S1 : s_word[4], sh.S2 = ONE ? w.S2 : s_word[5];
@@ -941,13 +943,13 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
                     o[4 * h + j].z += __uint_as_float(v[j][2]), o[4 * h + j].w += __uint_as_float(v[j][3]);
                   }
                 }
-                continue;
-              }
+              } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int row = r0 + s_row[tok * 32 + min(j0 + j, a.k - 1)];
-                const float4 u = __ldcg(reinterpret_cast<const float4*>(p0 + (long long)row * a.d));
-                o[j].x += u.x, o[j].y += u.y, o[j].z += u.z, o[j].w += u.w;
+                for (int j = 0; j < 8; ++j) {
+                  const int row = r0 + s_row[tok * 32 + min(j0 + j, a.k - 1)];
+                  const float4 u = __ldcg(reinterpret_cast<const float4*>(p0 + (long long)row * a.d));
+                  o[j].x += u.x, o[j].y += u.y, o[j].z += u.z, o[j].w += u.w;
+                }
               }
             }
 #pragma unroll
@@ -986,22 +988,22 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
       auto take = [&](float* sum, uint32_t at, const float* f) {
         if constexpr (ONE) {
           sum[0] = fmaf(tmem_read1(at), f[0], sum[0]);
-          return;
-        }
+        } else {
 #pragma unroll
-        for (int m = 0; m < NT; m += 16) {
-          if (m >= rows) break;
-          uint32_t v[16];
-          tmem_load16(at + m, v);
-          tmem_wait16(v);
-          const float4* f4 = reinterpret_cast<const float4*>(f + m);
+          for (int m = 0; m < NT; m += 16) {
+            if (m >= rows) break;
+            uint32_t v[16];
+            tmem_load16(at + m, v);
+            tmem_wait16(v);
+            const float4* f4 = reinterpret_cast<const float4*>(f + m);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 x = f4[q];
-            sum[m + 4 * q] = fmaf(__uint_as_float(v[4 * q]), x.x, sum[m + 4 * q]);
-            sum[m + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), x.y, sum[m + 4 * q + 1]);
-            sum[m + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), x.z, sum[m + 4 * q + 2]);
-            sum[m + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), x.w, sum[m + 4 * q + 3]);
+            for (int q = 0; q < 4; ++q) {
+              const float4 x = f4[q];
+              sum[m + 4 * q] = fmaf(__uint_as_float(v[4 * q]), x.x, sum[m + 4 * q]);
+              sum[m + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), x.y, sum[m + 4 * q + 1]);
+              sum[m + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), x.z, sum[m + 4 * q + 2]);
+              sum[m + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), x.w, sum[m + 4 * q + 3]);
+            }
           }
         }
       };

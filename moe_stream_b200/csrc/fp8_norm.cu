@@ -306,10 +306,14 @@ static cudaError_t launch_vec(const NormArgs& a, int sms, cudaStream_t s) {
     int threads = 32;
     while (threads < 512 && threads * (DT == DT_F32 ? 2 : 4) < chunks) threads *= 2;
     const int nc = (chunks + threads - 1) / threads;
-    if (threads == 32) return launch_tpr<DT, 32, NORM, true>(a, 32, nc, sms, s);
-    if (threads == 64) return launch_tpr<DT, 64, NORM, true>(a, 64, nc, sms, s);
-    if (threads == 128) return launch_tpr<DT, 128, NORM, true>(a, 128, nc, sms, s);
-    if (threads == 256) return launch_tpr<DT, 256, NORM, true>(a, 256, nc, sms, s);
+    if constexpr (DT == DT_F32) {              // below 512 threads: one or two chunks
+      if (threads < 512) return launch_tpr<DT, 0, NORM, true>(a, threads, nc, sms, s);
+    } else {
+      if (threads == 32) return launch_tpr<DT, 32, NORM, true>(a, 32, nc, sms, s);
+      if (threads == 64) return launch_tpr<DT, 64, NORM, true>(a, 64, nc, sms, s);
+      if (threads == 128) return launch_tpr<DT, 128, NORM, true>(a, 128, nc, sms, s);
+      if (threads == 256) return launch_tpr<DT, 256, NORM, true>(a, 256, nc, sms, s);
+    }
     return launch_tpr<DT, 512, NORM, true>(a, 512, nc, sms, s);
   }
   const int nc = (chunks + 511) / 512;
