@@ -133,9 +133,17 @@ __device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
 
 // 1 / sqrt(m), rounded once to 32 bits: two Newton steps in 64 from the 32-bit
 // estimate (relative error below 1e-13, far below half a step of the result),
-// a few instructions where the 64-bit root and quotient take many.
-__device__ __forceinline__ float rms_factor(double m) {
-  if (!(m > 1e-37 && m < 1e37)) return (float)(1.0 / sqrt(m));
+// a few instructions where the 64-bit root and quotient take many. Where the
+// factor of a row of very small or very large values is no normal 32-bit number,
+// *pre, a power of two that the values are multiplied with first, takes part of it.
+__device__ __forceinline__ float rms_factor(double m, float* pre) {
+  *pre = 1.f;
+  if (!(m > 1e-37 && m < 1e37)) {
+    double r = 1.0 / sqrt(m);
+    if (r < 1e-37) *pre = 0x1p-64f, r *= 0x1p64;
+    if (r > 1e37) *pre = 0x1p64f, r *= 0x1p-64;
+    return (float)r;
+  }
   double y = (double)rsqrtf((float)m);
 #pragma unroll
   for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-m * y, y, 1.0), y);
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__(TPR ? TPR : 512) k_norm_fp8(NormArgs a) {
     if (!PIPE) fetch(t);
     Raw<DT> h[NC];
     double ss = 0.0;
-    float f = 1.f;
+    float f = 1.f, pre = 1.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) h[i] = nx[i];
     if constexpr (NORM) {
@@ -219,7 +227,7 @@ __global__ void __launch_bounds__(TPR ? TPR : 512) k_norm_fp8(NormArgs a) {
         for (int i = 0; i < 16; ++i)
           if (i < warps) ss += red[turn][i];
       }
-      f = rms_factor(fma(ss, inv_d, a.eps));
+      f = rms_factor(fma(ss, inv_d, a.eps), &pre);
     }
     uint8_t* q = a.q + t * a.q_stride;
     float* s_row = a.s + (long long)t * groups + (threadIdx.x >> 4);
@@ -233,6 +241,9 @@ __global__ void __launch_bounds__(TPR ? TPR : 512) k_norm_fp8(NormArgs a) {
         float g[8] = {};
         if constexpr (PIPE) unpack<DT>(w[i], g);
         else if (mine) unpack<DT>(load8<DT, VEC>(static_cast<const E*>(a.w), c, d), g);
+        if (pre != 1.f)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= pre;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           mul2(v[j], v[j + 1], f, f);
