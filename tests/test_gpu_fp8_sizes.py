@@ -49,3 +49,33 @@ def test_row_counts_beyond_the_limit(lib, cuda):
                 bad()
     q2, s2 = fp8.quantize_fp8(one)
     assert torch.equal(q2.double(), q.double()) and torch.equal(s2, s)
+
+
+@pytest.mark.parametrize("M", [2, 15, 16, 17, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257])
+@pytest.mark.parametrize("N,K", [(256, 256), (257, 1025), (640, 1152)])
+def test_linear_around_the_tiles(M, N, K, lib, cuda):
+    """Row counts on both sides of every tile of the kernels and of the choice
+    between them."""
+    from moe_stream_b200 import fp8
+    from test_gpu_fp8 import check_linear
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    kb = -(-K // 128)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    xs = torch.rand(M, kb, generator=g, device="cuda") + 0.5
+    ws = (torch.rand(-(-N // 128), kb, generator=g, device="cuda") + 0.5) * 2.0 ** -12
+    check_linear(fp8.Fp8Linear(w, ws)(x, xs, out_dtype=torch.float32), x, xs, w, ws, None, "fp32")
+
+
+@pytest.mark.parametrize("model", ["qwen3", "gptoss"])
+@pytest.mark.parametrize("T", [2, 3, 4, 5, 11, 12, 13, 15, 16, 17, 31, 32, 33, 63, 64])
+def test_moe_around_the_tiles(model, T, lib, cuda):
+    """Token counts on both sides of every choice: routing by each CTA or
+    shared out, tokens of a route CTA, rows of an expert's tile."""
+    from test_gpu_fp8 import check_moe, make_moe
+    g = torch.Generator(device="cuda").manual_seed(T)
+    layer, router, rb, parts = make_moe(g, model, 320, 272, 24, 4)
+    x = torch.randn(T, 320, generator=g, device="cuda").to(torch.bfloat16)
+    y = layer(x)
+    check_moe(y, x, router, rb, parts, 4, model)
+    for _ in range(3):
+        assert torch.equal(layer(x), y)
