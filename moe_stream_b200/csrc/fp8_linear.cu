@@ -622,10 +622,12 @@ static cudaError_t launch_out(const LinearArgs& a, int sms, cudaStream_t s) {
   if (a.M <= 64) return launch_few<64, OUT>(a, sms, s);
   // Beyond 64 rows: the first kernel while its 128 x 64 tiles leave room to
   // cut a long K between CTAs, then single CTAs while their 128 x 128 tiles fit
-  // the GPU at once, then pairs (us, in this order: M 128, N 2880, K 4096 11.7,
-  // 16.2, 19.6; M 512, N 1024, K 4096 11.6, 16.2, 19.8; M 333, N 5120, K 2880
-  // 20.1, 13.3, 16.0; M 128, N 5120, K 2048 12.0, 10.0, 12.1; M 512, N 5120, K
-  // 2880 35.4, 22.3, 16.3; K 512 a draw of the first two).
+  // the GPU at once, then pairs (us, in this order: M 128, N 2880, K 4096 12.0,
+  // 16.6, 20.1; M 512, N 1024, K 4096 11.8, 16.2, 19.8; M 384, N 5120, K 2880
+  // 20.4, 13.6, 16.4; M 512, N 5120, K 2880 35.8, 22.6, 16.7; M 128, N 2880, K
+  // 1024 6.6, 6.1, 8.0, K 1536 7.5, 7.9, 9.8, K 512 5.8, 4.5, 6.3). Of 104
+  // shapes, N 1024 to 5120, K 512 to 4096, M 96 to 4096, the one chosen is
+  // within 6 % of the best but for N 1024, K 1024 (M 96 5.9 against 5.0).
   const long long rows = (a.N + 127) / 128;
   if (a.K > 1024 && 2 * rows * ((a.M + 63) / 64) <= sms) return launch_few<64, OUT>(a, sms, s);
   if (rows * ((a.M + 127) / 128) <= sms) return launch_rows<OUT, false>(a, sms, s);
