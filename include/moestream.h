@@ -435,9 +435,10 @@ int ms_rms_norm_fp8(const ms_fp8_norm* args, void* stream);
 
 /* y[m][n] = sum_b x_scales[m][b] w_scales[n/128][b]
  *           sum_{k in block b} x[m][k] w[n][k]  (+ bias[n]),
- * sums in 32 bits, one rounding to out_dtype. Rows of x and w start on
- * 16-byte boundaries (pad the stride when K is not a multiple of 16; what
- * lies between K and the stride is not used). */
+ * sums in 32 bits, one rounding to out_dtype. The product of the two scales is
+ * taken first, in 32 bits: it has to stay in their normal range, but for blocks
+ * of zeros. Rows of x and w start on 16-byte boundaries (pad the stride when K
+ * is not a multiple of 16; what lies between K and the stride is not used). */
 typedef struct ms_fp8_linear {
   const void* x;            /* e4m3 [M, K]                                         */
   const float* x_scales;    /* [M, ceil(K/128)]                                    */

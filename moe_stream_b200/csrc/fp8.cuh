@@ -5,7 +5,7 @@
 // consecutive features (the last group of a row may be shorter), weights one
 // per 128 x 128 block. The quantiser's scales are powers of two, so dividing
 // by one is exact and a code depends on the value alone; the products take
-// any fp32 scale.
+// any fp32 scales whose products stay in the normal range of 32 bits.
 #pragma once
 #include "ms_common.cuh"
 

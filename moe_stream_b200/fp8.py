@@ -14,7 +14,8 @@ in HBM whole. They chain as a decoder layer does:
 A matrix is (codes, scales): codes float8_e4m3fn, scales float32, one per row
 and 128 features of activations, one per 128 x 128 block of weights (e4m3
 code times scale is the value). The quantiser's scales are powers of two; the
-products take any scale.
+products take any scales whose products, a row's with a weight block's, stay in
+the normal range of 32 bits.
 
 Everything is asynchronous on the current stream of the inputs' device (or on
 ``stream=``, which the caller has made to wait for the inputs), allocates only through torch, keeps no state between calls and
