@@ -135,13 +135,15 @@ __device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
 // estimate (relative error below 1e-13, far below half a step of the result),
 // a few instructions where the 64-bit root and quotient take many. Where the
 // factor of a row of very small or very large values is no normal 32-bit number,
-// *pre, a power of two that the values are multiplied with first, takes part of it.
+// *pre, a power of two that the values are multiplied with first, takes part of
+// it (a row of zeros may leave more, where any finite factor does).
 __device__ __forceinline__ float rms_factor(double m, float* pre) {
   *pre = 1.f;
   if (!(m > 1e-37 && m < 1e37)) {
     double r = 1.0 / sqrt(m);
     if (r < 1e-37) *pre = 0x1p-64f, r *= 0x1p64;
     if (r > 1e37) *pre = 0x1p64f, r *= 0x1p-64;
+    if (m > 0.0) r = fmin(r, 1e38);
     return (float)r;
   }
   double y = (double)rsqrtf((float)m);

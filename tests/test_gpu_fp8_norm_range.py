@@ -32,3 +32,16 @@ def test_norm_over_the_whole_range(dt, T, d, eps, lib, cuda):
     e = yx.abs() * 3.01 * O.U32 + 2.0 ** -147
     check_codes(q, s, yx, e)
     assert ((y.double() - yx).abs() <= yx.abs() * HALF[dt] + TINIEST[dt] + 1.01 * e).all()
+
+
+@pytest.mark.parametrize("T,d", [(3, 130), (605, 10000)])
+@pytest.mark.parametrize("eps", [1e-6, 1e-60, 1e-100, 1e-200, 1e-300])
+def test_rows_of_zeros(T, d, eps, lib, cuda):
+    """0 / sqrt(eps) is 0, however small eps is; without one it is NaN."""
+    from moe_stream_b200 import fp8
+    for dt in DT.values():
+        x, w = torch.zeros(T, d, dtype=dt, device="cuda"), torch.ones(d, dtype=dt, device="cuda")
+        q, s, h, y = fp8.rms_norm_fp8(x, w, eps=eps, with_norm=True)
+        assert (y == 0).all() and (q.float() == 0).all() and (s == 2.0 ** -108).all()
+        q, s, h, y = fp8.rms_norm_fp8(x, w, eps=0.0, with_norm=True)
+        assert torch.isnan(y).all() and torch.isnan(q.float()).all() and torch.isnan(s).all() and (h == 0).all()
