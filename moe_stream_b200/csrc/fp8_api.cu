@@ -197,6 +197,14 @@ std::mutex g_answers_mutex;
 int* g_answers[16];
 int g_n_answers = 0;
 
+// What this thread does is no part of a capture, another thread's included: that
+// one stays whole though this one allocates or loads a kernel meanwhile.
+struct BesideCaptures {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 int* take_answer() {
   {
     std::lock_guard<std::mutex> lock(g_answers_mutex);
@@ -231,6 +239,7 @@ extern "C" int ms_fp8_status(int device, int* status, void* stream) {
   cudaError_t e = cudaStreamIsCapturing(s, &capturing);
   if (e != cudaSuccess || capturing != cudaStreamCaptureStatusNone)
     return bad(MS_E_INVALID, "%s: not for use in a capture", me);
+  BesideCaptures beside;
   int* at[2] = {};
   if (linear_fp8_status(&at[0]) != cudaSuccess || moe_fp8_status(&at[1]) != cudaSuccess)
     return bad(MS_E_CUDA, "%s: the status words have no address", me);

@@ -131,3 +131,38 @@ def test_tensors_dropped_after_the_call(lib, cuda):
         for a, b in zip(got, want):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), make.__name__
         del spoilt, got, want
+
+
+def test_a_stream_inside_a_capture(lib, cuda):
+    """stream= names a stream that has joined the capture: its calls are part of
+    the graph, and tensors dropped in between stay what they were."""
+    from moe_stream_b200 import fp8
+    g = _gen(4)
+    T, d, N = 9, 512, 640
+    x, r = (torch.randn(T, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    n = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(torch.bfloat16)
+    first, second = fp8.Fp8Linear(*_weight(g, N, d)), fp8.Fp8Linear(*_weight(g, d, N))
+    router, parts = _moe(g, d)
+    layer = fp8.Fp8MoELayer("qwen3", router, *parts, top_k=2)
+
+    def chain(**kw):
+        q, s, h = fp8.rms_norm_fp8(x, n, residual=r, **kw)
+        y = first(q, s, **kw)
+        q, s = fp8.quantize_fp8(y, **kw)
+        y = second(q, s, **kw)
+        q, s, h, y = fp8.rms_norm_fp8(y, n, residual=h, with_norm=True, **kw)
+        return layer(y, residual=h, **kw)
+
+    want = chain()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        a = chain(stream=side)
+        b = chain()                       # beside it
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(5):
+        a.fill_(7.0), b.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)

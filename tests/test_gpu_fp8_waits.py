@@ -181,3 +181,36 @@ def test_status_is_refused_in_a_capture(lib, cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+def test_status_beside_another_threads_capture():
+    """The first question of a process, which sets up the answer's memory, while
+    another thread captures: both go through. In a child process, as it has to be
+    the first."""
+    code = textwrap.dedent(f"""
+        import sys, threading
+        sys.path[:0] = [{ROOT!r}, {os.path.join(ROOT, 'tests')!r}]
+        import torch
+        from moe_stream_b200 import fp8
+        from test_gpu_fp8_waits import make_layer, tokens
+        g = torch.Generator(device="cuda").manual_seed(1)
+        layer, x = make_layer(g), tokens(g, 5)
+        want, side = layer(x), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        graph, said = torch.cuda.CUDAGraph(), []
+        def ask():
+            try:
+                fp8.status(0, stream=side)
+                said.append("ok")
+            except Exception as e:
+                said.append(repr(e))
+        with torch.cuda.graph(graph, capture_error_mode="global"):
+            t = threading.Thread(target=ask)
+            t.start(), t.join()
+            y = layer(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        print("RESULT", said, torch.equal(y, want))
+    """)
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert "RESULT ['ok'] True" in out.stdout, out.stdout[-500:] + out.stderr[-1500:]
