@@ -51,14 +51,16 @@ def _stream(device, stream=None):
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
-def _on_stream(call, stream, device, *args, keep=()):
-    """call(*args) with `stream` current: the tensors it makes belong to the
-    stream that writes them. The tensors it reads (args, and `keep`) may be
-    dropped once it returns: their memory is not used again before `stream`
-    has come past the call."""
+def _on_stream(call, stream, device, *args, keep=(), captured=None):
+    """call(*args) with `stream` current, behind the event `captured`: the
+    tensors it makes belong to the stream that writes them. The tensors it
+    reads (args, and `keep`) may be dropped once it returns: their memory is
+    not used again before `stream` has come past the call."""
     if stream.device.index != device:
         raise ValueError(f"stream is on {stream.device}, the inputs on cuda:{device}")
     with torch.cuda.stream(stream):
+        if captured is not None and torch.cuda.is_current_stream_capturing():
+            stream.wait_event(captured)
         out = call(*args)
     for t in (*args, *keep):
         if isinstance(t, torch.Tensor):
@@ -251,11 +253,13 @@ def _weight(name, codes, scales, rank, device=None):
 def _wait_for_copies(device, given, used):
     """Calls may come on any stream, so the copies that a constructor has
     queued are waited for. Inside a capture they are part of the graph, and so
-    are the calls that may read them."""
+    are the calls that may read them: the event behind them is returned."""
     if any(u is not None and u.data_ptr() != g.data_ptr() for g, u in zip(given, used)):
         with torch.cuda.device(device):
-            if not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream().synchronize()
+            if torch.cuda.is_current_stream_capturing():
+                return torch.cuda.current_stream().record_event()
+            torch.cuda.current_stream().synchronize()
+    return None
 
 
 class Fp8Linear:
@@ -281,7 +285,7 @@ class Fp8Linear:
         self.weight = w
         self.bias = _bias(bias, (N,), w.device)
         self.device = w.device
-        _wait_for_copies(w.device, (weight, scales, bias), (w, self.scales, self.bias))
+        self._captured = _wait_for_copies(w.device, (weight, scales, bias), (w, self.scales, self.bias))
         self._w = (w.data_ptr(), self.scales.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
         self._ld = _row_stride(w)
         self._dims = (K, N, _blocks(K), w.get_device())
@@ -292,7 +296,7 @@ class Fp8Linear:
         bf16, fp16 or fp32."""
         if stream is not None:
             return _on_stream(self._forward, stream, self.device.index, q, scales, out_dtype, out,
-                              keep=(self.weight, self.scales, self.bias))
+                              keep=(self.weight, self.scales, self.bias), captured=self._captured)
         return self._forward(q, scales, out_dtype, out)
 
     def _forward(self, q, scales, out_dtype, out):
@@ -373,8 +377,8 @@ class Fp8MoELayer:
             parts.append((self._aligned(codes), scales, _bias(m[2] if len(m) > 2 else None, (E, n), self.device)))
         self.gate, self.up, self.down = parts
         given = [t for m in (gate, up, down) for t in (*m[:2], m[2] if len(m) > 2 else None)]
-        _wait_for_copies(self.device, (router, router_bias, *given),
-                         (self.router, self.router_bias, *(t for p in parts for t in p)))
+        self._captured = _wait_for_copies(self.device, (router, router_bias, *given),
+                                          (self.router, self.router_bias, *(t for p in parts for t in p)))
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         self._ptrs = (*(ptr(p[0]) for p in parts), *(ptr(p[1]) for p in parts), *(ptr(p[2]) for p in parts))
         self._router = (ptr(self.router), ptr(self.router_bias))
@@ -403,7 +407,8 @@ class Fp8MoELayer:
         may be x or residual."""
         if stream is not None:
             return _on_stream(self._forward, stream, self.device.index, x, residual, out,
-                              keep=(self.router, self.router_bias, *self.gate, *self.up, *self.down))
+                              keep=(self.router, self.router_bias, *self.gate, *self.up, *self.down),
+                              captured=self._captured)
         return self._forward(x, residual, out)
 
     def _forward(self, x, residual, out):

@@ -67,8 +67,10 @@ def test_copies_made_by_a_constructor(lib, cuda):
 
 
 def test_constructors_in_a_capture(lib, cuda):
-    """Copies made in a capture belong to its graph, with the calls that read them."""
+    """Copies made in a capture belong to its graph, with the calls that read
+    them, on its stream and on one that has joined."""
     from moe_stream_b200 import fp8
+    side = torch.cuda.Stream()
     g = _gen(2)
     q, s = fp8.quantize_fp8(torch.randn(5, 512, generator=g, device="cuda"))
     w, ws = _weight(g, 640, 512)
@@ -77,10 +79,16 @@ def test_constructors_in_a_capture(lib, cuda):
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        y = fp8.Fp8Linear(*moved)(q, s)
-    graph.replay()
-    torch.cuda.synchronize()
-    assert torch.equal(y, want)
+        side.wait_stream(torch.cuda.current_stream())
+        torch.cuda._sleep(DELAY)
+        lin = fp8.Fp8Linear(*moved)
+        y, z = lin(q, s), lin(q, s, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        y.fill_(7.0), z.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, want)
 
 
 def test_tensors_dropped_after_the_call(lib, cuda):
@@ -141,7 +149,8 @@ def test_a_stream_inside_a_capture(lib, cuda):
     T, d, N = 9, 512, 640
     x, r = (torch.randn(T, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
     n = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(torch.bfloat16)
-    first, second = fp8.Fp8Linear(*_weight(g, N, d)), fp8.Fp8Linear(*_weight(g, d, N))
+    bias = torch.randn(N, generator=g, device="cuda").to(torch.bfloat16)      # copied
+    first, second = fp8.Fp8Linear(*_weight(g, N, d), bias), fp8.Fp8Linear(*_weight(g, d, N))
     router, parts = _moe(g, d)
     layer = fp8.Fp8MoELayer("qwen3", router, *parts, top_k=2)
 
