@@ -190,12 +190,17 @@ __global__ void k_take_status(int* linear, int* moe, volatile int* answer) {
   answer[1] = atomicExch(moe, 0);
 }
 
-// Pinned words for an answer, kept from call to call: two ints each, mapped on
-// every device. Those of a call that gave up waiting are not used again, as
-// its kernel may yet write them.
+// Pinned words for an answer, mapped on every device: two ints, and while they
+// are not in use the next free ones. They are kept from call to call (freeing
+// them would wait for the device), as many as calls were ever under way at once;
+// those of a call that gave up waiting are not used again, as its kernel may
+// yet write them.
+struct Answer {
+  int st[2];
+  Answer* next;
+};
 std::mutex g_answers_mutex;
-int* g_answers[16];
-int g_n_answers = 0;
+Answer* g_answers = nullptr;
 
 // What this thread does is no part of a capture, another thread's included: that
 // one stays whole though this one allocates or loads a kernel meanwhile.
@@ -205,25 +210,24 @@ struct BesideCaptures {
   ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-int* take_answer() {
+Answer* take_answer() {
   {
     std::lock_guard<std::mutex> lock(g_answers_mutex);
-    if (g_n_answers) return g_answers[--g_n_answers];
+    if (Answer* a = g_answers) {
+      g_answers = a->next;
+      return a;
+    }
   }
   void* p = nullptr;
-  if (cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) return static_cast<int*>(p);
+  if (cudaHostAlloc(&p, sizeof(Answer), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess)
+    return static_cast<Answer*>(p);
   cudaGetLastError();
   return nullptr;
 }
-void give_answer(int* a) {
-  {
-    std::lock_guard<std::mutex> lock(g_answers_mutex);
-    if (g_n_answers < 16) {
-      g_answers[g_n_answers++] = a;
-      return;
-    }
-  }
-  cudaFreeHost(a);
+void give_answer(Answer* a) {
+  std::lock_guard<std::mutex> lock(g_answers_mutex);
+  a->next = g_answers;
+  g_answers = a;
 }
 
 }  // namespace
@@ -247,14 +251,14 @@ extern "C" int ms_fp8_status(int device, int* status, void* stream) {
   e = stream_wait_bounded(s);
   int st[2] = {};
   if (e == cudaSuccess) {
-    int* answer = take_answer();
+    Answer* answer = take_answer();
     if (!answer) return bad(MS_E_CUDA, "%s: no pinned memory for the answer", me);
-    k_take_status<<<1, 1, 0, s>>>(at[0], at[1], answer);
+    k_take_status<<<1, 1, 0, s>>>(at[0], at[1], answer->st);
     e = cudaGetLastError();
     const bool asked = e == cudaSuccess;
     if (asked) e = stream_wait_bounded(s);
     if (e == cudaSuccess) {
-      const volatile int* v = answer;
+      const volatile int* v = answer->st;
       st[0] = v[0], st[1] = v[1];
     }
     if (e == cudaSuccess || !asked) give_answer(answer);
